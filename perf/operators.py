@@ -36,11 +36,11 @@ def listed():
         # a feed-forward's weight at load
         {"name": "quantise, a weight", "op": "quant_weight", "rows": 3072, "dim": 768, "type": "bf16"},
         # one query's projection: few rows, a whole weight to read
-        {"name": "product, one query", "op": "linear", "rows": 38, "dim": 768, "out": 768, "bias": True, "gelu": False},
+        {"name": "product, one query", "op": "linear", "rows": 38, "dim": 768, "out": 768, "bias": True, "gelu": False, "dtype": "bf16"},
         # the 1601 region classes of 16 images: an odd width
-        {"name": "product, region classes", "op": "linear", "rows": 1616, "dim": 1024, "out": 1601, "bias": True, "gelu": False},
+        {"name": "product, region classes", "op": "linear", "rows": 1616, "dim": 1024, "out": 1601, "bias": True, "gelu": False, "dtype": "bf16"},
         # an image stream's projection for 1024 images
-        {"name": "product, image batch", "op": "linear", "rows": 103424, "dim": 1024, "out": 1024, "bias": True, "gelu": False},
+        {"name": "product, image batch", "op": "linear", "rows": 103424, "dim": 1024, "out": 1024, "bias": True, "gelu": False, "dtype": "bf16"},
         # the text stream's first feed-forward product for 1024 queries, which stays in 8 bits
         {"name": "product to 8-bit, text batch", "op": "linear8", "rows": 38912, "dim": 768, "out": 3072, "bias": True, "gelu": True},
         # norm, product with GELU, product: a feed-forward of 64 queries as it is used
@@ -63,6 +63,8 @@ def draw(rng):
             if m * n <= 1.1e8 and m * n * k <= 1.0e11:
                 break
         case.update(rows=m, dim=k, out=n, bias=rng.random() < 0.7, gelu=rng.random() < 0.4)
+        if op == "linear":
+            case["dtype"] = "bf16" if rng.random() < 0.8 else "f32"
     elif op == "ffn":
         while True:
             m, k, n = _size(rng, 1, 40000), _size(rng, 32, 2048), _size(rng, 64, 8192)
@@ -158,18 +160,18 @@ def _grouped(y):
 
 
 def _scaled(y):
-    """y over its groups' scales as they are held, and the scales."""
+    """y over its groups' scales, and the scales."""
     v = _grouped(y)
-    scales = (v.abs().amax(-1) / E4M3_MAX).clamp(min=SCALE_MIN).bfloat16()
-    return (v * (1 / scales.to(v.dtype))[..., None]).flatten(-2)[..., : y.shape[-1]], scales
+    scales = (v.abs().amax(-1) / E4M3_MAX).clamp(min=SCALE_MIN)
+    return (v * (1 / scales)[..., None]).flatten(-2)[..., : y.shape[-1]], scales
 
 
 def _scaled_weight(w):
     n, k = w.shape
     v = torch.nn.functional.pad(w, (0, _ceil(k, BLOCK) * BLOCK - k, 0, _ceil(n, BLOCK) * BLOCK - n))
     v = v.view(_ceil(n, BLOCK), BLOCK, _ceil(k, BLOCK), BLOCK)
-    scales = (v.abs().amax((1, 3)) / E4M3_MAX).clamp(min=SCALE_MIN).bfloat16()
-    v = v * (1 / scales.to(v.dtype))[:, None, :, None]
+    scales = (v.abs().amax((1, 3)) / E4M3_MAX).clamp(min=SCALE_MIN)
+    v = v * (1 / scales)[:, None, :, None]
     return v.flatten(2).flatten(0, 1)[:n, :k], scales
 
 
@@ -234,7 +236,7 @@ def _own(s):
     op = case["op"]
     if op == "linear":
         return {"y": F_ops.fp8_block_linear(
-            s["x8"], s["xs"], s["w8"], s["ws"], s["b"], gelu=case["gelu"])}
+            s["x8"], s["xs"], s["w8"], s["ws"], s["b"], gelu=case["gelu"], out_dtype=TYPES[case["dtype"]])}
     if op == "linear8":
         q, scales = F_ops.fp8_block_linear_fp8(s["x8"], s["xs"], s["w8"], s["ws"], s["b"], gelu=case["gelu"])
         return {"q": q, "scales": scales}
@@ -269,7 +271,7 @@ def _plain(s):
     op = case["op"]
     if op in ("linear", "linear8"):
         y = _product(s["x8"], s["xs"], s["w8"], s["ws"], s["b"], case["gelu"], f)
-        return {"y": y.bfloat16()} if op == "linear" else dict(zip(("q", "scales"), _quantise(y)))
+        return {"y": y.to(TYPES[case["dtype"]])} if op == "linear" else dict(zip(("q", "scales"), _quantise(y)))
     if op == "ffn":
         total = _sum(s["x"], s["res"], f)
         q, scales = _quantise(_rms(total, s["w"].to(f))[0])
@@ -297,7 +299,7 @@ def _plain(s):
 
 @torch.no_grad()
 def exact(case, seed):
-    """64 bits; a value that is held in 8 bits, and its scale, stand here before they are rounded."""
+    """64 bits; a value that is held in 8 bits stands here before it is rounded."""
     s, f = prepare(case, seed), torch.float64
     op = case["op"]
 
@@ -343,9 +345,8 @@ def exact(case, seed):
         return {**dict(zip(("q", "scales"), by_groups(y))), **more}
     if op == "ffn":  # between the products the values are rounded as they are held, so that what is left is the last product's
         def held(v):
-            scales = by_groups(v)[1].bfloat16()
-            at = torch.arange(v.shape[-1], device="cuda") // BLOCK
-            return (v / scales.to(f)[:, at]).float().to(torch.float8_e4m3fn), scales
+            q, scales = by_groups(v)
+            return q.float().to(torch.float8_e4m3fn), scales
 
         q, scales = held(product(*held(y), s["w8"], s["ws"], s["b"], True))
         return {"y": product(q, scales, s["v8"], s["vs"], s["c"], False), **more}
@@ -363,22 +364,22 @@ def work(case):
     groups = _ceil(k, BLOCK)
     if op in ("linear", "linear8"):
         n = case["out"]
-        read = m * k + n * k + 2 * (m * groups + _ceil(n, BLOCK) * groups) + (2 * n if case["bias"] else 0)
-        write = m * n + 2 * m * _ceil(n, BLOCK) if op == "linear8" else 2 * m * n
+        read = m * k + n * k + 4 * (m * groups + _ceil(n, BLOCK) * groups) + (2 * n if case["bias"] else 0)
+        write = m * n + 4 * m * _ceil(n, BLOCK) if op == "linear8" else m * n * TYPES[case["dtype"]].itemsize
         return {"bytes": read + write, "flops": 2 * m * n * k}
     if op == "ffn":
         n = case["inner"]
-        weights = 2 * n * k + 4 * _ceil(n, BLOCK) * groups + 2 * (n + 2 * k)
+        weights = 2 * n * k + 8 * _ceil(n, BLOCK) * groups + 2 * (n + 2 * k)
         return {"bytes": 2 * 4 * m * k + weights, "flops": 4 * m * n * k}
     size = TYPES[case["type"]].itemsize
     if op == "quant_weight":
-        return {"bytes": m * k * (size + 1) + 2 * _ceil(m, BLOCK) * groups, "flops": 2 * m * k}
+        return {"bytes": m * k * (size + 1) + 4 * _ceil(m, BLOCK) * groups, "flops": 2 * m * k}
     if op == "quant":
-        return {"bytes": m * k * (size + 1) + 2 * m * groups, "flops": 2 * m * k}
+        return {"bytes": m * k * (size + 1) + 4 * m * groups, "flops": 2 * m * k}
     res = bool(case["residual"])
     if op == "rms8":
-        return {"bytes": m * k * (size * (1 + 2 * res) + 1) + 2 * m * groups + k * size, "flops": 6 * m * k}
+        return {"bytes": m * k * (size * (1 + 2 * res) + 1) + 4 * m * groups + k * size, "flops": 6 * m * k}
     if op == "layer8":
-        return {"bytes": m * k * (size * (2 + res) + 1) + 2 * m * groups + 2 * k * size, "flops": 10 * m * k}
+        return {"bytes": m * k * (size * (2 + res) + 1) + 4 * m * groups + 2 * k * size, "flops": 10 * m * k}
     # forward: x (and the residual) in, y (and the sum) out; backward: gy (and the sum's) in, x's out, the stream once more
     return {"bytes": m * k * size * (5 + 3 * res) + 3 * k * size, "flops": 14 * m * k}
