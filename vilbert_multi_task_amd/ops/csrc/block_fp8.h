@@ -1,13 +1,13 @@
-// 8-bit (OCP e4m3) values with one bf16 scale per block of 128: what the norms,
-// the quantisers and the products that share this format have in common.
+// 8-bit (OCP e4m3) values with one scale per block of 128, in bf16 or f32: what the
+// norms, the quantisers and the products that share this format have in common.
 //
-//   a = max |v| over the block's finite v    s = bf16(max(a / 448, 2^-100))
+//   a = max |v| over the block's finite v    s = held(max(a / 448, 2^-100))
 //   q = e4m3(v * (1 / s)), to nearest even   v ~ q * s
 //
-// A scale has bf16's 8 bits because more would say nothing: q is computed with
-// the scale as it is held, so its rounding is no error of the value. It moves
-// the largest |q| by 2^-8, to 449.75 at most, which still rounds to 448. The
-// product of two scales is exact in f32.
+// A scale in bf16 is half the bytes, and q is computed with the scale as it is
+// held, so that its rounding is hardly an error of the value: only where it went
+// down, a block's largest |q| comes to 449.75 at most and is stored as 448, 0.4%
+// less. In f32 the scale is a / 448 itself and the largest |q| is 448.
 // A value that is not finite is stored as e4m3's NaN and leaves its block's
 // scale alone, so it reaches the results that it belongs to and no others.
 // 2^-100 keeps 1/s finite where a block is all zeros.
@@ -64,14 +64,17 @@ DEV unsigned int pack2_bf16(float a, float b) {
   return __builtin_bit_cast(unsigned int, r);
 }
 
-// the scale of a block, as it is held, from its largest value
-DEV float block_scale(float amax) {
+// the scale of a block, as it is held in f32 or in bf16, from its largest value
+DEV float block_scale(float amax, bool f32) {
   const float s = fmaxf(amax / 448.0f, 0x1p-100f);
-  return us2f((unsigned short)pack2_bf16(s, s));
+  return f32 ? s : us2f((unsigned short)pack2_bf16(s, s));
 }
-DEV void store_scale(bf16* p, float scale) {  // of block_scale: nothing to round
-  *reinterpret_cast<unsigned short*>(p) =
-      (unsigned short)(__float_as_uint(scale) >> 16);
+// number i of `scales`, of block_scale: nothing to round
+DEV void store_scale(void* scales, long i, float scale, bool f32) {
+  if (f32)
+    ((float*)scales)[i] = scale;
+  else
+    ((unsigned short*)scales)[i] = (unsigned short)(__float_as_uint(scale) >> 16);
 }
 
 DEV void load8u(const bf16* p, float* out) {

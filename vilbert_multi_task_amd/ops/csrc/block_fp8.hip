@@ -34,11 +34,12 @@ struct NormArgs {
   const T *x, *res, *w, *b;
   T *y, *sum;
   unsigned char* y8;
-  bf16* scales;
+  void* scales;  // bf16, or f32 where scales_f32
   float* rstd;
   long rows;
   int dim;
   float eps;
+  bool scales_f32;
 };
 
 // us for 103424 rows of 1024 in bf16 (TB/s of what has to be moved): rms with the
@@ -119,11 +120,12 @@ __global__ __launch_bounds__(threads_of(L)) void block_norm_kernel(
       }
       if (FORM != kRms8) store8_row(a.y + row * dim, j, dim, y);
       if (FORM != kRms) {
-        const float scale = block_scale(group16_max(absmax<8>(y)));
+        const float scale = block_scale(group16_max(absmax<8>(y)), a.scales_f32);
         if (j < dim) {
           *reinterpret_cast<uint2*>(a.y8 + row * pitch + j) =
               pack8_block(y, 1.0f / scale);
-          if ((t & 15) == 0) store_scale(a.scales + row * groups + j / kBlock, scale);
+          if ((t & 15) == 0)
+            store_scale(a.scales, row * groups + j / kBlock, scale, a.scales_f32);
         }
       }
     }
@@ -135,7 +137,7 @@ __global__ __launch_bounds__(threads_of(L)) void block_norm_kernel(
 template <typename T>
 __global__ __launch_bounds__(256) void quantize_block_kernel(
     const T* __restrict__ x, unsigned char* __restrict__ y8,
-    bf16* __restrict__ scales, long rows, int dim) {
+    void* __restrict__ scales, bool scales_f32, long rows, int dim) {
   const int groups = ceil_div(dim, kBlock);
   const long pitch = fp8_pitch(dim);
   const long n = rows * groups;
@@ -145,10 +147,10 @@ __global__ __launch_bounds__(256) void quantize_block_kernel(
     const int j = (int)(g - row * groups) * kBlock + (threadIdx.x & 15) * 8;
     float v[8];
     load8_row(x + row * dim, j, dim, v);
-    const float scale = block_scale(group16_max(absmax<8>(v)));
+    const float scale = block_scale(group16_max(absmax<8>(v)), scales_f32);
     if (j < dim)
       *reinterpret_cast<uint2*>(y8 + row * pitch + j) = pack8_block(v, 1.0f / scale);
-    if ((threadIdx.x & 15) == 0) store_scale(scales + g, scale);
+    if ((threadIdx.x & 15) == 0) store_scale(scales, g, scale, scales_f32);
   }
 }
 
@@ -157,7 +159,7 @@ __global__ __launch_bounds__(256) void quantize_block_kernel(
 template <typename T>
 __global__ __launch_bounds__(256) void quantize_block_weight_kernel(
     const T* __restrict__ w, unsigned char* __restrict__ w8,
-    bf16* __restrict__ scales, int n, int k) {
+    void* __restrict__ scales, bool scales_f32, int n, int k) {
   __shared__ float lds[4];
   const long pitch = fp8_pitch(k);
   const int j = blockIdx.x * kBlock + (threadIdx.x & 15) * 8;
@@ -176,7 +178,7 @@ __global__ __launch_bounds__(256) void quantize_block_weight_kernel(
   if (lane_id() == 0) lds[wave_id()] = a;
   __syncthreads();
   const float scale =
-      block_scale(fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3])));
+      block_scale(fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3])), scales_f32);
   const float inv = 1.0f / scale;
 #pragma unroll
   for (int r = 0; r < 8; ++r) {
@@ -185,7 +187,7 @@ __global__ __launch_bounds__(256) void quantize_block_weight_kernel(
       *reinterpret_cast<uint2*>(w8 + row * pitch + j) = pack8_block(v[r], inv);
   }
   if (threadIdx.x == 0)
-    store_scale(scales + (long)blockIdx.y * gridDim.x + blockIdx.x, scale);
+    store_scale(scales, (long)blockIdx.y * gridDim.x + blockIdx.x, scale, scales_f32);
 }
 
 // Backward of y = n * w, n = t * rstd:  h = gy * w,  c = mean(h * n),
@@ -337,9 +339,10 @@ void norm_by_width(const NormArgs<T>& a, hipStream_t stream) {
 template <typename T>
 void launch_block_norm(int form, const T* x, const T* res, const T* w,
                        const T* b, T* y, T* sum, unsigned char* y8,
-                       bf16* scales, float* rstd, long rows, int dim,
-                       float eps, hipStream_t stream) {
-  const NormArgs<T> a{x, res, w, b, y, sum, y8, scales, rstd, rows, dim, eps};
+                       void* scales, bool scales_f32, float* rstd, long rows,
+                       int dim, float eps, hipStream_t stream) {
+  const NormArgs<T> a{x,    res,  w,   b,   y,  sum,
+                      y8, scales, rstd, rows, dim, eps, scales_f32};
   if (form == 0)
     res ? norm_by_width<T, kRms, true>(a, stream)
         : norm_by_width<T, kRms, false>(a, stream);
@@ -384,33 +387,35 @@ void launch_rms_bwd(const T* gy, const T* gsum, const T* t, const float* rstd,
 }
 
 template <typename T>
-void launch_quantize_block(const T* x, unsigned char* y8, bf16* scales,
-                           long rows, int dim, hipStream_t stream) {
+void launch_quantize_block(const T* x, unsigned char* y8, void* scales,
+                           bool scales_f32, long rows, int dim,
+                           hipStream_t stream) {
   const long blocks = (rows * ceil_div(dim, kBlock) + 15) / 16;
   hipLaunchKernelGGL((quantize_block_kernel<T>),
                      dim3((int)(blocks < 8192 ? blocks : 8192)), dim3(256), 0,
-                     stream, x, y8, scales, rows, dim);
+                     stream, x, y8, scales, scales_f32, rows, dim);
 }
 
 template <typename T>
-void launch_quantize_block_weight(const T* w, unsigned char* w8, bf16* scales,
-                                  int n, int k, hipStream_t stream) {
+void launch_quantize_block_weight(const T* w, unsigned char* w8, void* scales,
+                                  bool scales_f32, int n, int k,
+                                  hipStream_t stream) {
   hipLaunchKernelGGL((quantize_block_weight_kernel<T>),
                      dim3(ceil_div(k, kBlock), ceil_div(n, kBlock)), dim3(256),
-                     0, stream, w, w8, scales, n, k);
+                     0, stream, w, w8, scales, scales_f32, n, k);
 }
 
 #define INSTANTIATE(T)                                                        \
   template void launch_block_norm<T>(int, const T*, const T*, const T*,       \
                                      const T*, T*, T*, unsigned char*,        \
-                                     bf16*, float*, long, int, float,         \
+                                     void*, bool, float*, long, int, float,   \
                                      hipStream_t);                            \
   template void launch_rms_bwd<T>(const T*, const T*, const T*, const float*, \
                                   const T*, T*, T*, float*, long, int,        \
                                   hipStream_t);                               \
-  template void launch_quantize_block<T>(const T*, unsigned char*, bf16*,     \
-                                         long, int, hipStream_t);             \
-  template void launch_quantize_block_weight<T>(const T*, unsigned char*,     \
-                                                bf16*, int, int, hipStream_t);
+  template void launch_quantize_block<T>(const T*, unsigned char*, void*,     \
+                                         bool, long, int, hipStream_t);       \
+  template void launch_quantize_block_weight<T>(                              \
+      const T*, unsigned char*, void*, bool, int, int, hipStream_t);
 INSTANTIATE(bf16)
 INSTANTIATE(float)

@@ -16,17 +16,17 @@ using bf16 = __hip_bfloat16;
 
 template <typename T>
 void launch_block_norm(int form, const T*, const T*, const T*, const T*, T*, T*,
-                       unsigned char*, bf16*, float*, long, int, float,
+                       unsigned char*, void*, bool, float*, long, int, float,
                        hipStream_t);
 int rms_bwd_parts(long rows, int dim);
 template <typename T>
 void launch_rms_bwd(const T*, const T*, const T*, const float*, const T*, T*,
                     T*, float*, long, int, hipStream_t);
 template <typename T>
-void launch_quantize_block(const T*, unsigned char*, bf16*, long, int,
+void launch_quantize_block(const T*, unsigned char*, void*, bool, long, int,
                            hipStream_t);
 template <typename T>
-void launch_quantize_block_weight(const T*, unsigned char*, bf16*, int, int,
+void launch_quantize_block_weight(const T*, unsigned char*, void*, bool, int, int,
                                   hipStream_t);
 void launch_block_gemm(const unsigned char*, const bf16*, const unsigned char*,
                        const bf16*, const void*, bool, void*, bf16*, long, long,
@@ -83,10 +83,10 @@ at::Tensor empty_rows8(at::IntArrayRef sizes, const at::Tensor& like) {
   auto y = fresh(s, at::kFloat8_e4m3fn, like);
   return s.back() == k ? y : y.narrow(-1, 0, k);
 }
-at::Tensor empty_scales(at::IntArrayRef sizes, const at::Tensor& like) {
+at::Tensor empty_scales(at::IntArrayRef sizes, const at::Tensor& like, bool f32) {
   at::DimVector s(sizes.begin(), sizes.end());
   s.back() = ceil_to(s.back(), kBlock);
-  return fresh(s, at::kBFloat16, like);
+  return fresh(s, f32 ? at::kFloat : at::kBFloat16, like);
 }
 unsigned char* bytes(const at::Tensor& t) { return (unsigned char*)t.data_ptr(); }
 bf16* scales_of(const at::Tensor& t) { return (bf16*)t.data_ptr(); }
@@ -110,7 +110,8 @@ void norm_as(int form, const at::Tensor& x, const OptTensor& res,
   launch_block_norm<T>(
       form, (const T*)x.data_ptr(), ptr<T>(res), (const T*)w.data_ptr(),
       ptr<T>(b), (T*)ptr<T>(y), (T*)ptr<T>(sum),
-      (unsigned char*)ptr<unsigned char>(y8), (bf16*)ptr<bf16>(scales),
+      (unsigned char*)ptr<unsigned char>(y8), (void*)ptr<void>(scales),
+      scales.has_value() && scales->scalar_type() == at::kFloat,
       (float*)ptr<float>(rstd), rows, (int)x.size(-1), (float)eps, cur_stream());
   C10_HIP_KERNEL_LAUNCH_CHECK();
 }
@@ -252,12 +253,12 @@ std::tuple<at::Tensor, at::Tensor> rms_norm_residual_autograd(
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_fp8_block(
     const at::Tensor& x_in, const OptTensor& res, const at::Tensor& w,
-    double eps) {
+    double eps, bool f32_scales) {
   check_norm("rms_norm_fp8_block", x_in, res, w);
   c10::DeviceGuard guard(x_in.device());
   const auto x = x_in.contiguous();
   auto y8 = empty_rows8(x.sizes(), x);
-  auto scales = empty_scales(x.sizes(), x);
+  auto scales = empty_scales(x.sizes(), x, f32_scales);
   auto sum = res.has_value() ? fresh_like(x) : fresh({0}, x.scalar_type(), x);
   norm(1, x, dense(res), w.contiguous(), {}, {}, res.has_value() ? OptTensor(sum) : OptTensor(),
        y8, scales, {}, eps);
@@ -266,7 +267,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_fp8_block(
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_fp8_block(
     const at::Tensor& x_in, const OptTensor& res, const at::Tensor& w,
-    const at::Tensor& b, double eps) {
+    const at::Tensor& b, double eps, bool f32_scales) {
   const char* op = "layer_norm_fp8_block";
   check_norm(op, x_in, res, w);
   check_like(op, "bias", x_in, b, false);
@@ -274,26 +275,26 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_fp8_block(
   const auto x = x_in.contiguous();
   auto y = fresh_like(x);
   auto y8 = empty_rows8(x.sizes(), x);
-  auto scales = empty_scales(x.sizes(), x);
+  auto scales = empty_scales(x.sizes(), x, f32_scales);
   norm(2, x, dense(res), w.contiguous(), b.contiguous(), y, {}, y8, scales, {},
        eps);
   return {y, y8, scales};
 }
 
-std::tuple<at::Tensor, at::Tensor> quantize_fp8_block(const at::Tensor& x_in) {
+std::tuple<at::Tensor, at::Tensor> quantize_fp8_block(const at::Tensor& x_in,
+                                                      bool f32_scales) {
   const long rows = rows_of("quantize_fp8_block", x_in);
   c10::DeviceGuard guard(x_in.device());
   const auto x = x_in.contiguous();
   auto y8 = empty_rows8(x.sizes(), x);
-  auto scales = empty_scales(x.sizes(), x);
+  auto scales = empty_scales(x.sizes(), x, f32_scales);
   if (rows) {
     if (x.scalar_type() == at::kFloat)
-      launch_quantize_block<float>(x.data_ptr<float>(), bytes(y8),
-                                   scales_of(scales), rows,
-                                   (int)x.size(-1), cur_stream());
+      launch_quantize_block<float>(x.data_ptr<float>(), bytes(y8), scales.data_ptr(),
+                                   f32_scales, rows, (int)x.size(-1), cur_stream());
     else
       launch_quantize_block<bf16>((const bf16*)x.data_ptr(), bytes(y8),
-                                  scales_of(scales), rows,
+                                  scales.data_ptr(), f32_scales, rows,
                                   (int)x.size(-1), cur_stream());
     C10_HIP_KERNEL_LAUNCH_CHECK();
   }
@@ -301,7 +302,7 @@ std::tuple<at::Tensor, at::Tensor> quantize_fp8_block(const at::Tensor& x_in) {
 }
 
 std::tuple<at::Tensor, at::Tensor> quantize_fp8_block_weight(
-    const at::Tensor& w_in) {
+    const at::Tensor& w_in, bool f32_scales) {
   const char* op = "quantize_fp8_block_weight";
   const long rows = rows_of(op, w_in);
   TORCH_CHECK(w_in.dim() == 2, op, ": a weight has two dimensions, got ",
@@ -311,15 +312,15 @@ std::tuple<at::Tensor, at::Tensor> quantize_fp8_block_weight(
   const auto w = w_in.contiguous();
   auto w8 = empty_rows8(w.sizes(), w);
   auto scales = fresh({ceil_to(rows, kBlock), ceil_to(w.size(1), kBlock)},
-                      at::kBFloat16, w);
+                      f32_scales ? at::kFloat : at::kBFloat16, w);
   if (rows) {
     if (w.scalar_type() == at::kFloat)
       launch_quantize_block_weight<float>(w.data_ptr<float>(), bytes(w8),
-                                          scales_of(scales), (int)rows,
+                                          scales.data_ptr(), f32_scales, (int)rows,
                                           (int)w.size(1), cur_stream());
     else
       launch_quantize_block_weight<bf16>((const bf16*)w.data_ptr(), bytes(w8),
-                                         scales_of(scales), (int)rows,
+                                         scales.data_ptr(), f32_scales, (int)rows,
                                          (int)w.size(1), cur_stream());
     C10_HIP_KERNEL_LAUNCH_CHECK();
   }
@@ -433,7 +434,7 @@ std::tuple<at::Tensor, at::Tensor> fp8_block_linear_fp8(
   c10::DeviceGuard guard(x8.device());
   const Product p = product(op, x8, xs, w8, ws, bias);
   auto y8 = empty_rows8(p.sizes, x8);
-  auto scales = empty_scales(p.sizes, x8);
+  auto scales = empty_scales(p.sizes, x8, false);
   launch(p, y8.data_ptr(), scales_of(scales), gelu);
   return {y8, scales};
 }
@@ -463,10 +464,10 @@ struct Serving<R(A...), f, name> {
 TORCH_LIBRARY_FRAGMENT(vilbert_amd, m) {
   m.def("rms_norm(Tensor x, Tensor w, float eps) -> Tensor");
   m.def("rms_norm_residual(Tensor x, Tensor res, Tensor w, float eps) -> (Tensor, Tensor)");
-  m.def("rms_norm_fp8_block(Tensor x, Tensor? res, Tensor w, float eps) -> (Tensor, Tensor, Tensor)");
-  m.def("layer_norm_fp8_block(Tensor x, Tensor? res, Tensor w, Tensor b, float eps) -> (Tensor, Tensor, Tensor)");
-  m.def("quantize_fp8_block(Tensor x) -> (Tensor, Tensor)");
-  m.def("quantize_fp8_block_weight(Tensor w) -> (Tensor, Tensor)");
+  m.def("rms_norm_fp8_block(Tensor x, Tensor? res, Tensor w, float eps, bool f32_scales=False) -> (Tensor, Tensor, Tensor)");
+  m.def("layer_norm_fp8_block(Tensor x, Tensor? res, Tensor w, Tensor b, float eps, bool f32_scales=False) -> (Tensor, Tensor, Tensor)");
+  m.def("quantize_fp8_block(Tensor x, bool f32_scales=False) -> (Tensor, Tensor)");
+  m.def("quantize_fp8_block_weight(Tensor w, bool f32_scales=False) -> (Tensor, Tensor)");
   m.def("fp8_block_linear(Tensor x8, Tensor x_scales, Tensor w8, Tensor w_scales, Tensor? bias, bool gelu) -> Tensor");
   m.def("fp8_block_linear_fp8(Tensor x8, Tensor x_scales, Tensor w8, Tensor w_scales, Tensor? bias, bool gelu) -> (Tensor, Tensor)");
 }

@@ -572,8 +572,9 @@ def _rms(t, weight, eps):
 
 
 # --------------------------------------------------------------------------
-# 8-bit (e4m3) rows with one bf16 scale per block of 128 values. Per block:
-#   s = bf16(max(max |v| / 448, 2^-100)),  q = e4m3(v * (1 / s))
+# 8-bit (e4m3) rows with one scale per block of 128 values, in bf16 (half the
+# bytes) or in f32 as `scale_dtype` says. Per block:
+#   s = scale_dtype(max(max |v| / 448, 2^-100)),  q = e4m3(v * (1 / s))
 # A value that is not finite becomes e4m3's NaN and leaves the block's scale
 # alone. Nothing is kept between calls. On the GPU 8-bit rows begin at
 # multiples of 16 bytes (a view where the width is no such multiple).
@@ -600,19 +601,25 @@ def _serve_hip(op: str, *tensors: Optional[torch.Tensor]) -> bool:
     return False
 
 
-def quantize_fp8_block(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+def quantize_fp8_block(
+    x: torch.Tensor, scale_dtype: torch.dtype = torch.bfloat16
+) -> Tuple[torch.Tensor, torch.Tensor]:
     """x [..., K] (bf16/f32) -> (x8 [..., K] e4m3, scales [..., ceil(K/128)])."""
+    f32 = _f32_scales("quantize_fp8_block", scale_dtype)
     if _serve_hip("quantize_fp8_block", x):
-        return _EXT.quantize_fp8_block(x)
+        return _EXT.quantize_fp8_block(x, f32)
     _check_rows("quantize_fp8_block", x)
-    return _quantize_block_ref(x.float())
+    return _quantize_block_ref(x.float(), scale_dtype)
 
 
-def quantize_fp8_block_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+def quantize_fp8_block_weight(
+    w: torch.Tensor, scale_dtype: torch.dtype = torch.bfloat16
+) -> Tuple[torch.Tensor, torch.Tensor]:
     """w [N, K] (bf16/f32) in blocks of 128 x 128 ->
     (w8 [N, K] e4m3, scales [ceil(N/128), ceil(K/128)])."""
+    f32 = _f32_scales("quantize_fp8_block_weight", scale_dtype)
     if _serve_hip("quantize_fp8_block_weight", w):
-        return _EXT.quantize_fp8_block_weight(w)
+        return _EXT.quantize_fp8_block_weight(w, f32)
     _check_rows("quantize_fp8_block_weight", w)
     if w.dim() != 2:
         raise RuntimeError(f"quantize_fp8_block_weight: a weight has two dimensions, got {w.dim()}")
@@ -621,7 +628,7 @@ def quantize_fp8_block_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tens
     v = torch.nn.functional.pad(
         w.float(), (0, kb * FP8_BLOCK - k, 0, nb * FP8_BLOCK - n)
     ).view(nb, FP8_BLOCK, kb, FP8_BLOCK)
-    q, scales = _quantize_ref(v, (1, 3))
+    q, scales = _quantize_ref(v, (1, 3), scale_dtype)
     return q.reshape(nb * FP8_BLOCK, kb * FP8_BLOCK)[:n, :k], scales.view(nb, kb)
 
 
@@ -630,16 +637,18 @@ def rms_norm_fp8_block(
     weight: torch.Tensor,
     eps: float,
     residual: Optional[torch.Tensor] = None,
+    scale_dtype: torch.dtype = torch.bfloat16,
 ):
     """rms_norm whose y leaves in 8 bits, quantised from its f32 values:
     (y8, scales), and with a residual (y8, scales, x + residual)."""
+    f32 = _f32_scales("rms_norm_fp8_block", scale_dtype)
     if _serve_hip("rms_norm_fp8_block", x, weight, residual):
         y8, scales, total = _EXT.rms_norm_fp8_block(
-            x, residual, weight, eps)
+            x, residual, weight, eps, f32)
         return (y8, scales) if residual is None else (y8, scales, total)
     _check_norm("rms_norm_fp8_block", x, weight, residual)
     t = x if residual is None else x + residual
-    y8, scales = _quantize_block_ref(_rms(t, weight, eps))
+    y8, scales = _quantize_block_ref(_rms(t, weight, eps), scale_dtype)
     return (y8, scales) if residual is None else (y8, scales, t)
 
 
@@ -649,17 +658,19 @@ def layer_norm_fp8_block(
     bias: torch.Tensor,
     eps: float,
     residual: Optional[torch.Tensor] = None,
+    scale_dtype: torch.dtype = torch.bfloat16,
 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """layer_norm(x + residual) in x's dtype and in 8 bits, both from the same
     f32 values: (y, y8, scales). Rows of up to 65536 values."""
+    f32 = _f32_scales("layer_norm_fp8_block", scale_dtype)
     if _serve_hip("layer_norm_fp8_block", x, weight, bias, residual):
         return _EXT.layer_norm_fp8_block(
-            x, residual, weight, bias, eps)
+            x, residual, weight, bias, eps, f32)
     _check_norm("layer_norm_fp8_block", x, weight, residual, bias)
     t = x.float() if residual is None else x.float() + residual.float()
     y = torch.nn.functional.layer_norm(
         t, (x.shape[-1],), weight.float(), bias.float(), eps)
-    return (y.to(x.dtype), *_quantize_block_ref(y))
+    return (y.to(x.dtype), *_quantize_block_ref(y, scale_dtype))
 
 
 def fp8_block_linear(
@@ -694,26 +705,26 @@ def fp8_block_linear_fp8(
     if _serve_hip("fp8_block_linear_fp8", x8, x_scales, w8, w_scales, bias):
         return _EXT.fp8_block_linear_fp8(x8, x_scales, w8, w_scales, bias, gelu)
     return _quantize_block_ref(_block_linear_ref(
-        "fp8_block_linear_fp8", x8, x_scales, w8, w_scales, bias, gelu))
+        "fp8_block_linear_fp8", x8, x_scales, w8, w_scales, bias, gelu), torch.bfloat16)
 
 
 # -- the plain forms of the above: the CPU path and the kernels' oracle ------
 
-def _quantize_ref(v: torch.Tensor, dims):
+def _quantize_ref(v: torch.Tensor, dims, scale_dtype):
     """v in blocks over `dims` -> (e4m3 like v, scales with those dims kept)."""
     a = v.abs()
     most = torch.where(torch.isfinite(a), a, 0.0).amax(dims, keepdim=True)
-    scales = (most / _E4M3_MAX).clamp(min=_SCALE_MIN).bfloat16()
+    scales = (most / _E4M3_MAX).clamp(min=_SCALE_MIN).to(scale_dtype)
     q = v * (1.0 / scales.float())
     q = torch.where(torch.isfinite(q), q, float("nan"))
     return q.to(torch.float8_e4m3fn), scales
 
 
-def _quantize_block_ref(y: torch.Tensor):
+def _quantize_block_ref(y: torch.Tensor, scale_dtype):
     k = y.shape[-1]
     kb = -(-k // FP8_BLOCK)
     v = torch.nn.functional.pad(y, (0, kb * FP8_BLOCK - k))
-    q, scales = _quantize_ref(v.unflatten(-1, (kb, FP8_BLOCK)), -1)
+    q, scales = _quantize_ref(v.unflatten(-1, (kb, FP8_BLOCK)), -1, scale_dtype)
     return q.flatten(-2)[..., :k], scales.squeeze(-1)
 
 
@@ -727,6 +738,14 @@ def _block_linear_ref(op, x8, x_scales, w8, w_scales, bias, gelu):
     if bias is not None:
         y = y + bias.float()
     return torch.nn.functional.gelu(y) if gelu else y
+
+
+def _f32_scales(op: str, scale_dtype: torch.dtype) -> bool:
+    if scale_dtype is torch.bfloat16:
+        return False
+    if scale_dtype is torch.float32:
+        return True
+    raise RuntimeError(f"{op}: scale_dtype must be bf16/f32, got {scale_dtype}")
 
 
 def _check_rows(op: str, x: torch.Tensor) -> None:
