@@ -28,9 +28,9 @@ void launch_quantize_block(const T*, unsigned char*, void*, bool, long, int,
 template <typename T>
 void launch_quantize_block_weight(const T*, unsigned char*, void*, bool, int, int,
                                   hipStream_t);
-void launch_block_gemm(const unsigned char*, const bf16*, const unsigned char*,
-                       const bf16*, const void*, bool, void*, bf16*, long, long,
-                       int, int, int, bool, hipStream_t);
+void launch_block_gemm(const unsigned char*, const void*, const unsigned char*,
+                       const void*, bool, const void*, bool, void*, bool, void*,
+                       long, long, int, int, int, bool, hipStream_t);
 
 namespace {
 
@@ -89,7 +89,6 @@ at::Tensor empty_scales(at::IntArrayRef sizes, const at::Tensor& like, bool f32)
   return fresh(s, f32 ? at::kFloat : at::kBFloat16, like);
 }
 unsigned char* bytes(const at::Tensor& t) { return (unsigned char*)t.data_ptr(); }
-bf16* scales_of(const at::Tensor& t) { return (bf16*)t.data_ptr(); }
 
 OptTensor dense(const OptTensor& t) {
   return t.has_value() ? OptTensor(t->contiguous()) : t;
@@ -369,10 +368,10 @@ Product product(const char* op, const at::Tensor& x8, const at::Tensor& xs,
                   w8.scalar_type() == at::kFloat8_e4m3fn,
               op, ": x8 and w8 must be float8_e4m3fn, got ", x8.scalar_type(),
               " and ", w8.scalar_type());
-  TORCH_CHECK(xs.scalar_type() == at::kBFloat16 &&
-                  ws.scalar_type() == at::kBFloat16,
-              op, ": scales must be bf16, got ", xs.scalar_type(), " and ",
-              ws.scalar_type());
+  TORCH_CHECK(xs.scalar_type() == ws.scalar_type() &&
+                  (xs.scalar_type() == at::kBFloat16 || xs.scalar_type() == at::kFloat),
+              op, ": scales must be both bf16 or both f32, got ", xs.scalar_type(),
+              " and ", ws.scalar_type());
   TORCH_CHECK(x8.dim() >= 1 && w8.dim() == 2 && x8.size(-1) == w8.size(1), op,
               ": x8 [..., K] and w8 [N, K] are needed, got ", x8.sizes(), " and ",
               w8.sizes());
@@ -404,25 +403,27 @@ Product product(const char* op, const at::Tensor& x8, const at::Tensor& xs,
   return {rows8(x8), rows8(w8), xs.contiguous(), ws.contiguous(), b, sizes, n, k};
 }
 
-void launch(const Product& p, void* y, bf16* ys, bool gelu) {
+bool f32_scales(const Product& p) { return p.xs.scalar_type() == at::kFloat; }
+void launch(const Product& p, const at::Tensor& y, void* ys, bool gelu) {
   if (p.x.rows == 0) return;
   launch_block_gemm(
-      bytes(p.x.t), scales_of(p.xs), bytes(p.w.t), scales_of(p.ws),
+      bytes(p.x.t), p.xs.data_ptr(), bytes(p.w.t), p.ws.data_ptr(), f32_scales(p),
       p.bias.defined() ? p.bias.data_ptr() : nullptr,
-      p.bias.defined() && p.bias.scalar_type() == at::kFloat, y, ys, p.x.pitch,
-      p.w.pitch, (int)p.x.rows, (int)p.n, (int)p.k, gelu, cur_stream());
+      p.bias.defined() && p.bias.scalar_type() == at::kFloat, y.data_ptr(),
+      y.scalar_type() == at::kFloat, ys, p.x.pitch, p.w.pitch, (int)p.x.rows,
+      (int)p.n, (int)p.k, gelu, cur_stream());
   C10_HIP_KERNEL_LAUNCH_CHECK();
 }
 
 at::Tensor fp8_block_linear(const at::Tensor& x8, const at::Tensor& xs,
                             const at::Tensor& w8, const at::Tensor& ws,
-                            const OptTensor& bias, bool gelu) {
+                            const OptTensor& bias, bool gelu, bool f32_out) {
   const char* op = "fp8_block_linear";
   TORCH_CHECK(x8.is_cuda(), op, ": a GPU tensor is needed");
   c10::DeviceGuard guard(x8.device());
   const Product p = product(op, x8, xs, w8, ws, bias);
-  auto y = fresh(p.sizes, at::kBFloat16, x8);
-  launch(p, y.data_ptr(), nullptr, gelu);
+  auto y = fresh(p.sizes, f32_out ? at::kFloat : at::kBFloat16, x8);
+  launch(p, y, nullptr, gelu);
   return y;
 }
 
@@ -434,8 +435,8 @@ std::tuple<at::Tensor, at::Tensor> fp8_block_linear_fp8(
   c10::DeviceGuard guard(x8.device());
   const Product p = product(op, x8, xs, w8, ws, bias);
   auto y8 = empty_rows8(p.sizes, x8);
-  auto scales = empty_scales(p.sizes, x8, false);
-  launch(p, y8.data_ptr(), scales_of(scales), gelu);
+  auto scales = empty_scales(p.sizes, x8, f32_scales(p));
+  launch(p, y8, scales.data_ptr(), gelu);
   return {y8, scales};
 }
 
@@ -468,7 +469,7 @@ TORCH_LIBRARY_FRAGMENT(vilbert_amd, m) {
   m.def("layer_norm_fp8_block(Tensor x, Tensor? res, Tensor w, Tensor b, float eps, bool f32_scales=False) -> (Tensor, Tensor, Tensor)");
   m.def("quantize_fp8_block(Tensor x, bool f32_scales=False) -> (Tensor, Tensor)");
   m.def("quantize_fp8_block_weight(Tensor w, bool f32_scales=False) -> (Tensor, Tensor)");
-  m.def("fp8_block_linear(Tensor x8, Tensor x_scales, Tensor w8, Tensor w_scales, Tensor? bias, bool gelu) -> Tensor");
+  m.def("fp8_block_linear(Tensor x8, Tensor x_scales, Tensor w8, Tensor w_scales, Tensor? bias, bool gelu, bool f32_out=False) -> Tensor");
   m.def("fp8_block_linear_fp8(Tensor x8, Tensor x_scales, Tensor w8, Tensor w_scales, Tensor? bias, bool gelu) -> (Tensor, Tensor)");
 }
 

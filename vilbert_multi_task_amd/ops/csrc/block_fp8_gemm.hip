@@ -11,8 +11,11 @@
 // What the instruction rounds: it aligns 8 neighbouring products to the largest
 // of them and drops what is below 2^-13 of it (measured; all e4m3 instructions
 // of this card do), the sums of eights are f32. On normal values that is 1.5e-5
-// of the result's 2-norm, a hundredth of bf16's step, so y leaves as bf16 or in
-// 8 bits; f32 results would promise more than there is.
+// of the result's 2-norm, with a few channels ten times as large 3e-5: a hundredth
+// of bf16's step, and less of an 8-bit one. Where something leaves in 32 bits, y
+// itself or the scales of an 8-bit y, the products are exact instead: e4m3 values
+// are bf16 values, and of those four 16x16x32 instructions take the block, twice as
+// long (measured: 1e-8 of the 2-norm for a block, 4e-8 for eight).
 //
 // W is the instruction's first operand and X its second: a lane's four results
 // are then four neighbouring outputs of ONE row of X, which is what a store, a
@@ -20,20 +23,22 @@
 // of a row; the order of the 128 products within the sum is the same for both,
 // whatever it is.
 
+#include <type_traits>
+
 #include "block_fp8.h"
 
 namespace {
 
 using i32x8 = __attribute__((ext_vector_type(8))) int;
 
-enum Out { kBf16, kFp8 };
+enum Out { kBf16, kFp8, kF32 };
 
 struct GemmArgs {
   const unsigned char *x, *w;  // rows at 16 bytes
-  const bf16 *xs, *ws;
+  const void *xs, *ws;         // of the kernel's type of scales
   const void* bias;  // or null; bf16, or f32 where bias_f32
   void* y;
-  bf16* ys;  // 8-bit output: its scales
+  void* ys;  // 8-bit output: its scales, of the type of the others
   long x_pitch, w_pitch;
   int m, n, k;
   bool gelu, bias_f32;
@@ -49,6 +54,51 @@ DEV float bias_at(const GemmArgs& a, int n) {
 DEV f32x4 mfma128(i32x8 a, i32x8 b) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
       a, b, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+}
+
+// SF: scales are f32, else bf16. What is read of one, and its value:
+template <bool SF>
+using Held = std::conditional_t<SF, unsigned, unsigned short>;
+template <bool SF>
+DEV float scale_value(unsigned held) {
+  return SF ? __uint_as_float(held) : us2f((unsigned short)held);
+}
+
+// What leaves in 32 bits has to be right in 32.
+template <Out OUT, bool SF>
+constexpr bool kExact = OUT == kF32 || (OUT == kFp8 && SF);
+
+// A lane's 32 values of one operand's row as the instructions take them: e4m3, or
+// bf16, into which e4m3 goes as it is, NaN included.
+using bf16v2 = __attribute__((ext_vector_type(2))) __bf16;
+using bf16v8 = __attribute__((ext_vector_type(8))) __bf16;
+struct Bf16x32 { bf16v8 v[4]; };
+template <bool EXACT>
+using Operand = std::conditional_t<EXACT, Bf16x32, i32x8>;
+template <bool EXACT>
+DEV Operand<EXACT> operand(i32x8 raw) {
+  if constexpr (EXACT) {
+    Bf16x32 to;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bf16v2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw[i], 1.f, false);
+      const bf16v2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw[i], 1.f, true);
+      const int at = i % 2 * 4;
+      to.v[i / 2][at] = a[0], to.v[i / 2][at + 1] = a[1];
+      to.v[i / 2][at + 2] = b[0], to.v[i / 2][at + 3] = b[1];
+    }
+    return to;
+  } else {
+    return raw;
+  }
+}
+DEV f32x4 block_product(const i32x8& a, const i32x8& b) { return mfma128(a, b); }
+DEV f32x4 block_product(const Bf16x32& a, const Bf16x32& b) {
+  f32x4 p = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[i], b.v[i], p, 0, 0, 0);
+  return p;
 }
 
 // 16 bytes of a row from column k on, k a multiple of 16; zero past its end.
@@ -79,7 +129,23 @@ DEV i32x8 load32_row(const unsigned char* row, int k, int dim) {
 // 3e-5, and to 1e-4 up to 6. |v| is bounded where |v| h is nothing, so that
 // infinities come out as the limits. The minimum and the maximum are those that
 // keep NaN, which also need no quieting of their operands.
+// For what leaves in 32 bits the fit has degree 14 and goes to |v| = 12.9, beyond which
+// h is no normal number of f32 and taken as 0: h is good to 1.3e-6 of itself up to 4,
+// 1.4e-5 up to 8, 1.3e-3 at the end.
+template <bool EXACT>
 DEV float gelu(float v) {
+  if constexpr (EXACT) {
+    constexpr float c[] = {5.91124225e-14f, -5.77921784e-12f, 2.54662189e-10f,
+                           -6.67860814e-9f, 1.15810212e-7f,   -1.3914505e-6f,
+                           1.17169952e-5f,  -6.68080758e-5f,  2.13216115e-4f,
+                           1.99831872e-4f,  -7.27495374e-3f,  5.27356344e-2f,
+                           0.45909019f,     1.15112632f,      0.99999939f};
+    const float a = __builtin_elementwise_minimum(fabsf(v), 14.f);
+    float p = c[0];
+#pragma unroll
+    for (int i = 1; i < 15; ++i) p = p * a + c[i];
+    return __builtin_elementwise_maximum(v, 0.f) - a * __builtin_amdgcn_exp2f(-p);
+  }
   const float a = __builtin_elementwise_minimum(fabsf(v), 16.f);
   float p = 1.7221218e-6f;
   p = p * a - 5.9576460e-5f;
@@ -116,7 +182,12 @@ DEV void store8_row(bf16* row, int j, int dim, uint4 v) {
         reinterpret_cast<unsigned short*>(row)[j + i] = w[i / 2] >> (16 * (i & 1));
   }
 }
-DEV void store4_row(bf16* row, int j, int dim, const float* v) {
+struct __attribute__((packed, aligned(4))) F32x4 { float f[4]; };
+DEV void store4(float* p, const float* v) {
+  *reinterpret_cast<F32x4*>(p) = {{v[0], v[1], v[2], v[3]}};
+}
+template <typename T>
+DEV void store4_row(T* row, int j, int dim, const float* v) {
   if (j + 4 <= dim) {
     store4(row + j, v);
   } else {
@@ -134,8 +205,9 @@ DEV void store4_row(bf16* row, int j, int dim, const float* v) {
 // next block's operands on their way while one is multiplied. Their sums are added
 // through shared memory, in the order of the waves. (An 8-bit result needs 128
 // outputs in one workgroup, and then reading them takes as long as with tiles.)
-template <int NT, int MT>
+template <int NT, int MT, Out OUT, bool SF>
 __global__ __launch_bounds__(512) void block_gemm_direct_kernel(GemmArgs a) {
+  constexpr bool EXACT = kExact<OUT, SF>;
   constexpr int KW = 8;
   static_assert(NT * MT <= KW, "a wave for each part of the result");
   __shared__ f32x4 part[KW][NT * MT][64];
@@ -147,7 +219,7 @@ __global__ __launch_bounds__(512) void block_gemm_direct_kernel(GemmArgs a) {
 
   // rows past the end are read as the last one and not written
   const unsigned char *wrow[NT], *xrow[MT];
-  const bf16* xs[MT];
+  const Held<SF>* xs[MT];
 #pragma unroll
   for (int t = 0; t < NT; ++t)
     wrow[t] = a.w + (long)min(n0 + t * 16 + r, a.n - 1) * a.w_pitch;
@@ -155,9 +227,9 @@ __global__ __launch_bounds__(512) void block_gemm_direct_kernel(GemmArgs a) {
   for (int u = 0; u < MT; ++u) {
     const long m = min(m0 + u * 16 + r, a.m - 1);
     xrow[u] = a.x + m * a.x_pitch;
-    xs[u] = a.xs + m * kb;
+    xs[u] = (const Held<SF>*)a.xs + m * kb;
   }
-  const bf16* const ws = a.ws + (long)(n0 / kBlock) * kb;
+  const Held<SF>* const ws = (const Held<SF>*)a.ws + (long)(n0 / kBlock) * kb;
 
   i32x8 w[NT], x[MT];
   float s[MT];
@@ -167,25 +239,25 @@ __global__ __launch_bounds__(512) void block_gemm_direct_kernel(GemmArgs a) {
     for (int t = 0; t < NT; ++t) w[t] = load32_row(wrow[t], k, a.k);
 #pragma unroll
     for (int u = 0; u < MT; ++u) x[u] = load32_row(xrow[u], k, a.k);
-    const float wsb = bf2f(ws[b]);
+    const float wsb = scale_value<SF>(ws[b]);
 #pragma unroll
-    for (int u = 0; u < MT; ++u) s[u] = bf2f(xs[u][b]) * wsb;
+    for (int u = 0; u < MT; ++u) s[u] = scale_value<SF>(xs[u][b]) * wsb;
   };
   f32x4 acc[NT][MT] = {};
   if (kw < kb) load(kw);
   for (int b = kw; b < kb; b += KW) {
-    i32x8 wb[NT], xb[MT];
+    Operand<EXACT> wb[NT], xb[MT];
     float sb[MT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) wb[t] = w[t];
+    for (int t = 0; t < NT; ++t) wb[t] = operand<EXACT>(w[t]);
 #pragma unroll
-    for (int u = 0; u < MT; ++u) xb[u] = x[u], sb[u] = s[u];
+    for (int u = 0; u < MT; ++u) xb[u] = operand<EXACT>(x[u]), sb[u] = s[u];
     if (b + KW < kb) load(b + KW);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int u = 0; u < MT; ++u) {
-        const f32x4 p = mfma128(wb[t], xb[u]);
+        const f32x4 p = block_product(wb[t], xb[u]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[t][u][i] += p[i] * sb[u];
       }
@@ -209,9 +281,10 @@ __global__ __launch_bounds__(512) void block_gemm_direct_kernel(GemmArgs a) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     v[i] += bias_at(a, n + i);
-    if (a.gelu) v[i] = gelu(v[i]);
+    if (a.gelu) v[i] = gelu<EXACT>(v[i]);
   }
-  store4_row((bf16*)a.y + (long)m * a.n, n, a.n, v);
+  using Y = std::conditional_t<OUT == kF32, float, bf16>;
+  store4_row((Y*)a.y + (long)m * a.n, n, a.n, v);
 }
 
 // --- tiles through shared memory ---------------------------------------------
@@ -289,15 +362,21 @@ DEV void stage_last(const unsigned char* base, const unsigned* off,
 // Where there are fewer tiles than compute units, KG = 2 such teams of waves share a
 // tile: each has every other block of the shared axis, buffers of its own, and the
 // second hands its sums to the first at the end.
-template <int WN, int WM, int MT, int KG, Out OUT>
-__global__ __launch_bounds__(KG * WN * WM * 64, MT == 4 ? 2 : MT == 2 ? 3 : 4) void
+template <int WN, int WM, int MT, int KG, Out OUT, bool SF>
+__global__ __launch_bounds__(KG * WN * WM * 64,
+                             MT == 4 || (MT == 2 && kExact<OUT, SF>) ? 2
+                             : MT == 2                               ? 3
+                                                                     : 4) void
 block_gemm_tile_kernel(GemmArgs a, int mtiles, int ntiles) {
+  constexpr bool EXACT = kExact<OUT, SF>;
   constexpr int T = WN * WM * 64;  // threads of a team
   constexpr int kN = WN * 128, kM = WM * MT * 16;
   constexpr int kStep = T / 8;  // rows that one load of all threads covers
   constexpr int kWLoads = kN / kStep, kXLoads = kM / kStep;
   // the fewer rows a wave has, the fewer instructions a step has to wait behind
-  constexpr int kParts = MT == 4 ? 2 : MT == 2 ? 3 : 4, kLag = MT == 1 ? 2 : 1;
+  // (exact products take four times the instructions, and registers, a step)
+  constexpr int kParts = EXACT || MT == 4 ? 2 : MT == 2 ? 3 : 4,
+                kLag = EXACT || MT != 1 ? 1 : 2;
   // one load every so many matrix instructions
   constexpr int kEvery = 8 * MT / (kWLoads + kXLoads);
   static_assert(kEvery >= 1, "each load has its place");
@@ -351,8 +430,8 @@ block_gemm_tile_kernel(GemmArgs a, int mtiles, int ntiles) {
   // it from there. Fetched block by block, 16 rows' lines each time for two bytes
   // of each, they cost as much of the first cache as half of X.
   const int group = min(n0 / kBlock + wn, groups - 1);
-  const unsigned short* const ws = (const unsigned short*)a.ws + (long)group * kb;
-  const unsigned short* const xs = (const unsigned short*)a.xs + (long)m0 * kb;
+  const Held<SF>* const ws = (const Held<SF>*)a.ws + (long)group * kb;
+  const Held<SF>* const xs = (const Held<SF>*)a.xs + (long)m0 * kb;
   unsigned xsoff[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t)
@@ -367,13 +446,13 @@ block_gemm_tile_kernel(GemmArgs a, int mtiles, int ntiles) {
 
   f32x4 acc[8][MT] = {};
   float s[MT];
-  i32x8 xf[MT];
+  Operand<EXACT> xf[MT];
   auto take_scales = [&](int b) __attribute__((always_inline)) {
     const int from = (b / KG & 3) * 16;
-    const float w = us2f(__builtin_amdgcn_readlane(ws4, from));
+    const float w = scale_value<SF>(__builtin_amdgcn_readlane(ws4, from));
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      s[t] = w * us2f(__builtin_amdgcn_ds_bpermute((from + r) * 4, xs4[t]));
+      s[t] = w * scale_value<SF>(__builtin_amdgcn_ds_bpermute((from + r) * 4, xs4[t]));
       // here and not later, where waiting for them would be waiting for W
       asm volatile("" : "+v"(s[t]));
     }
@@ -381,7 +460,8 @@ block_gemm_tile_kernel(GemmArgs a, int mtiles, int ntiles) {
   auto take_x = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < MT; ++t)
-      xf[t] = read_frag(ldsx + ((wm * MT + t) * 16 + r) * 128, q, swizzle_x(r));
+      xf[t] = operand<EXACT>(
+          read_frag(ldsx + ((wm * MT + t) * 16 + r) * 128, q, swizzle_x(r)));
   };
   auto w_at = [](int b) { return (b / KG & 1) * kN * 128; };
   // The loads of a block, one at a time: W's first, then X's.
@@ -406,17 +486,20 @@ block_gemm_tile_kernel(GemmArgs a, int mtiles, int ntiles) {
 #pragma unroll
     for (int t = 0; t < kParts; ++t) wf[t] = part(t);
 #pragma unroll
-    for (int t = 0; t < kLag; ++t)
+    for (int t = 0; t < kLag; ++t) {
+      const Operand<EXACT> w = operand<EXACT>(wf[t]);
 #pragma unroll
-      for (int u = 0; u < MT; ++u) p[t][u] = mfma128(wf[t], xf[u]);
+      for (int u = 0; u < MT; ++u) p[t][u] = block_product(w, xf[u]);
+    }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
       if (t + kParts < 8) wf[t % kParts] = part(t + kParts);
+      Operand<EXACT> w;
+      if (t + kLag < 8) w = operand<EXACT>(wf[(t + kLag) % kParts]);
 #pragma unroll
       for (int u = 0; u < MT; ++u) {
-        if (t + kLag < 8)
-          p[(t + kLag) % (kLag + 1)][u] = mfma128(wf[(t + kLag) % kParts], xf[u]);
+        if (t + kLag < 8) p[(t + kLag) % (kLag + 1)][u] = block_product(w, xf[u]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[t][u][i] += p[t % (kLag + 1)][u][i] * s[u];
         if ((t * MT + u) % kEvery == 0) between((t * MT + u) / kEvery);
@@ -494,12 +577,36 @@ block_gemm_tile_kernel(GemmArgs a, int mtiles, int ntiles) {
 #pragma unroll
       for (int u = 0; u < MT; ++u)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][u][i] = gelu(acc[t][u][i]);
+        for (int i = 0; i < 4; ++i) acc[t][u][i] = gelu<EXACT>(acc[t][u][i]);
+  }
+  if (nw >= a.n) return;
+  if constexpr (OUT == kF32) {
+    // Four lanes have a whole line of 128 bytes, and it goes past the caches (38912 x
+    // 3072 x 768: 254 us with plain stores, 243 with these).
+#pragma unroll
+    for (int u = 0; u < MT; ++u) {
+      const int m = m0 + (wm * MT + u) * 16 + r;
+      if (m >= a.m) continue;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int at = nw + g * 32 + q * 8;
+        float* const row = (float*)a.y + (long)m * a.n;
+        float v8[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v8[i] = acc[2 * g + i / 4][u][i & 3];
+        if (at + 8 <= a.n) {
+          store16_past(row + at, __builtin_bit_cast(uint4, acc[2 * g][u]));
+          store16_past(row + at + 4, __builtin_bit_cast(uint4, acc[2 * g + 1][u]));
+        } else {
+          ::store8_row(row, at, a.n, v8);
+        }
+      }
+    }
+    return;
   }
   // Out through shared memory, each wave through a part of its own, so that a
   // store instruction writes whole rows of 128 outputs. Pieces of 16 bytes change
   // places within a row by its number, as before.
-  if (nw >= a.n) return;
   unsigned char* const out = all + wave * (MT * 16 * 256);
 #pragma unroll
   for (int u = 0; u < MT; ++u) {
@@ -524,7 +631,7 @@ block_gemm_tile_kernel(GemmArgs a, int mtiles, int ntiles) {
       float most = absmax<32>(v);
       most = fmaxf(most, __shfl_xor(most, 16));
       most = fmaxf(most, __shfl_xor(most, 32));
-      const float scale = block_scale(most, false), inv = 1.0f / scale;
+      const float scale = block_scale(most, SF), inv = 1.0f / scale;
 #pragma unroll
       for (int g = 0; g < 4; ++g)
         *reinterpret_cast<uint2*>(out + row * 128 +
@@ -532,7 +639,7 @@ block_gemm_tile_kernel(GemmArgs a, int mtiles, int ntiles) {
             pack8_block(v + 8 * g, inv);
       const int m = m0 + wm * MT * 16 + row;
       if (q == 0 && m < a.m)
-        store_scale(a.ys, (long)m * groups + nw / kBlock, scale, false);
+        store_scale(a.ys, (long)m * groups + nw / kBlock, scale, SF);
     }
   }
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -553,20 +660,15 @@ block_gemm_tile_kernel(GemmArgs a, int mtiles, int ntiles) {
   }
 }
 
-template <int WN, int WM, int MT, int KG = 1>
+template <int WN, int WM, int MT, int KG, Out OUT, bool SF>
 void launch_tiles(const GemmArgs& a, hipStream_t stream) {
   constexpr int kLds = KG * (2 * WN * 128 * 128 + WM * MT * 16 * 128);
   static_assert(kLds >= WN * WM * MT * (16 * 256 + (KG - 1) * 8 * 1024),
                 "room for the results");
   const int mtiles = ceil_div(a.m, WM * MT * 16), ntiles = ceil_div(a.n, WN * 128);
-  if (a.ys)
-    hipLaunchKernelGGL((block_gemm_tile_kernel<WN, WM, MT, KG, kFp8>),
-                       dim3(mtiles * ntiles), dim3(KG * WN * WM * 64), kLds, stream, a,
-                       mtiles, ntiles);
-  else
-    hipLaunchKernelGGL((block_gemm_tile_kernel<WN, WM, MT, KG, kBf16>),
-                       dim3(mtiles * ntiles), dim3(KG * WN * WM * 64), kLds, stream, a,
-                       mtiles, ntiles);
+  hipLaunchKernelGGL((block_gemm_tile_kernel<WN, WM, MT, KG, OUT, SF>),
+                     dim3(mtiles * ntiles), dim3(KG * WN * WM * 64), kLds, stream, a,
+                     mtiles, ntiles);
 }
 
 // --- large products ----------------------------------------------------------
@@ -616,9 +718,10 @@ DEV void wide_load4(const void* base, unsigned offset, unsigned lds) {
 
 // Widths that are multiples of 128 both ways, from 256 outputs, 256 rows and two
 // blocks of the shared axis on.
-template <Out OUT>
+template <Out OUT, bool SF>
 __global__ __launch_bounds__(512, 2) void block_gemm_wide_kernel(GemmArgs a, int mtiles,
                                                                  int ntiles) {
+  static_assert(!kExact<OUT, SF>, "its registers are full as it is");
   constexpr int kTurn = 24;  // the instruction before which the barrier is
   extern __shared__ __attribute__((aligned(128))) unsigned char all[];
 
@@ -646,7 +749,7 @@ __global__ __launch_bounds__(512, 2) void block_gemm_wide_kernel(GemmArgs a, int
   // tiles; what its neighbour has is not written again.
   int lt = first, lb = 0, m1 = 0, n1 = 0;
   const unsigned char *wfrom = a.w, *xfrom = a.x;
-  const bf16 *sfrom = a.xs;
+  const Held<SF>* sfrom = nullptr;
   unsigned woff[4], xoff[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -656,7 +759,7 @@ __global__ __launch_bounds__(512, 2) void block_gemm_wide_kernel(GemmArgs a, int
                      (((tid & 7) ^ swizzle_x(tid / 8)) << 4));
   }
   // waves 0 to 3 load the rows' scales, 4 W's, and the others do so for nothing
-  const unsigned soff = opaque((wave < 4 ? tid : tid & 1) * kb * 2);
+  const unsigned soff = opaque((wave < 4 ? tid : tid & 1) * kb * (int)sizeof(Held<SF>));
   auto enter = [&]() __attribute__((always_inline)) {
     const int strip = lt / (16 * mtiles);
     const int width = min(16, ntiles - strip * 16);
@@ -666,7 +769,8 @@ __global__ __launch_bounds__(512, 2) void block_gemm_wide_kernel(GemmArgs a, int
     const int m0 = min(m1, a.m - 256), n0 = min(n1, a.n - 256);
     wfrom = a.w + n0 * a.w_pitch;
     xfrom = a.x + m0 * a.x_pitch;
-    sfrom = wave < 4 ? a.xs + (long)m0 * kb : a.ws + (long)(n0 / kBlock) * kb;
+    sfrom = wave < 4 ? (const Held<SF>*)a.xs + (long)m0 * kb
+                     : (const Held<SF>*)a.ws + (long)(n0 / kBlock) * kb;
   };
   auto next = [&]() __attribute__((always_inline)) {
     wfrom += kBlock;
@@ -683,7 +787,8 @@ __global__ __launch_bounds__(512, 2) void block_gemm_wide_kernel(GemmArgs a, int
     if (i == 1) wide_load16<8192>(xfrom, xoff[1], to);
     if (i == 2) wide_load16<16384>(xfrom, xoff[2], to);
     if (i == 3) wide_load16<24576>(xfrom, xoff[3], to);
-    if (i == 4) wide_load2(sfrom, soff, lds_s + buf * kWideScales);
+    if (i == 4 && SF) wide_load4(sfrom, soff, lds_s + buf * kWideScales);
+    if (i == 4 && !SF) wide_load2(sfrom, soff, lds_s + buf * kWideScales);
   };
   auto load_w = [&](const unsigned char* from, int i, int buf)
       __attribute__((always_inline)) {
@@ -722,7 +827,7 @@ __global__ __launch_bounds__(512, 2) void block_gemm_wide_kernel(GemmArgs a, int
   auto take_scales = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      s[u] = us2f((unsigned short)raw[4]) * us2f((unsigned short)raw[u]);
+      s[u] = scale_value<SF>(raw[4]) * scale_value<SF>(raw[u]);
   };
 
   enter();
@@ -814,7 +919,7 @@ __global__ __launch_bounds__(512, 2) void block_gemm_wide_kernel(GemmArgs a, int
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[t][u][i] = gelu(acc[t][u][i]);
+          for (int i = 0; i < 4; ++i) acc[t][u][i] = gelu<false>(acc[t][u][i]);
           __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -877,29 +982,22 @@ __global__ __launch_bounds__(512, 2) void block_gemm_wide_kernel(GemmArgs a, int
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was loaded past the last tile
 }
 
+template <Out OUT, bool SF>
 void launch_wide(const GemmArgs& a, hipStream_t stream) {
   const int mtiles = ceil_div(a.m, 256), ntiles = ceil_div(a.n, 256);
   const long tiles = (long)mtiles * ntiles;
   const dim3 grid((unsigned)(tiles < 256 ? tiles : 256));
-  if (a.ys)
-    hipLaunchKernelGGL((block_gemm_wide_kernel<kFp8>), grid, dim3(512), kWideLds, stream, a,
-                       mtiles, ntiles);
-  else
-    hipLaunchKernelGGL((block_gemm_wide_kernel<kBf16>), grid, dim3(512), kWideLds, stream, a,
-                       mtiles, ntiles);
+  hipLaunchKernelGGL((block_gemm_wide_kernel<OUT, SF>), grid, dim3(512), kWideLds, stream,
+                     a, mtiles, ntiles);
 }
 
-template <int NT, int MT>
+template <int NT, int MT, Out OUT, bool SF>
 void launch_direct(const GemmArgs& a, hipStream_t stream) {
   const dim3 grid(ceil_div(a.n, NT * 16) * ceil_div(a.m, 16 * MT));
-  hipLaunchKernelGGL((block_gemm_direct_kernel<NT, MT>), grid, dim3(512), 0,
+  hipLaunchKernelGGL((block_gemm_direct_kernel<NT, MT, OUT, SF>), grid, dim3(512), 0,
                      stream, a);
 }
 
-}  // namespace
-
-// y in bf16, or in e4m3 where `ys` takes its scales.
-//
 // The larger the tile the less is read for each result, as long as every compute
 // unit has a workgroup or two. us with bias to bf16 ("x2": two teams):
 //   rows x width x shared  direct 16x32  32x64  tiles 128x64 x2  128x64  128x128  256x128
@@ -924,31 +1022,54 @@ void launch_direct(const GemmArgs& a, hipStream_t stream) {
 //   38912 x 3072 x 768       7.13    124 / 141 / 100 / 124       116 / 138 / 96.5 / 134
 //   38912 x 3072 x 1536      7.13    204 / 214 / 178 / 201       186 / 201 / 167 / 205
 //   16384 x 4096 x 4096      4.00    272 / 263 / 245 / 255       231 / 232 / 213 / 237
-void launch_block_gemm(const unsigned char* x, const bf16* xs,
-                       const unsigned char* w, const bf16* ws,
-                       const void* bias, bool bias_f32, void* y, bf16* ys,
-                       long x_pitch, long w_pitch, int m, int n, int k,
-                       bool gelu, hipStream_t stream) {
-  const GemmArgs a{x,       w,       xs, ws, bias, y,    ys,
-                   x_pitch, w_pitch, m,  n,  k,    gelu, bias_f32};
+template <Out OUT, bool SF>
+void launch_best(const GemmArgs& a, hipStream_t stream) {
+  const int m = a.m, n = a.n, k = a.k;
   auto tiles = [&](long of_n, long of_m) {
     return ((n + of_n - 1) / of_n) * ((m + of_m - 1) / of_m);
   };
   constexpr long kUnits = 256;  // compute units
-  if (!ys && tiles(16, 32) <= 2 * kUnits)
-    return m <= 16 ? launch_direct<1, 1>(a, stream) : launch_direct<1, 2>(a, stream);
-  if (!ys && tiles(32, 64) <= kUnits) return launch_direct<2, 4>(a, stream);
-  if (tiles(128, 64) <= kUnits) return launch_tiles<1, 4, 1, 2>(a, stream);
-  if (tiles(128, 64) <= 2 * kUnits) return launch_tiles<1, 4, 1>(a, stream);
-  // 256 x 256 where workgroups come out about even, but not for GELU to 8 bits of a
-  // short shared axis: nothing runs beside its results' work
-  const long wide = tiles(256, 256), rounds = (wide + kUnits - 1) / kUnits;
-  if (k % kBlock == 0 && k >= 2 * kBlock && n % kBlock == 0 && n >= 256 && m >= 256 &&
-      4 * wide >= 3 * rounds * kUnits && !(ys && gelu && k < 2048))
-    return launch_wide(a, stream);
-  // 256 x 128 goes round twice a unit at a time: the last round has to be worth it
-  const long large = tiles(256, 128), round = 2 * kUnits;
-  if (large >= 4 * round || 10 * large >= 8 * ((large + round - 1) / round) * round)
-    return launch_tiles<2, 2, 4>(a, stream);
-  launch_tiles<1, 4, 2>(a, stream);
+  if constexpr (OUT != kFp8) {
+    if (tiles(16, 32) <= 2 * kUnits)
+      return m <= 16 ? launch_direct<1, 1, OUT, SF>(a, stream)
+                     : launch_direct<1, 2, OUT, SF>(a, stream);
+    if (tiles(32, 64) <= kUnits) return launch_direct<2, 4, OUT, SF>(a, stream);
+  }
+  if (tiles(128, 64) <= kUnits) return launch_tiles<1, 4, 1, 2, OUT, SF>(a, stream);
+  if (tiles(128, 64) <= 2 * kUnits) return launch_tiles<1, 4, 1, 1, OUT, SF>(a, stream);
+  if constexpr (!kExact<OUT, SF>) {
+    // 256 x 256 where workgroups come out about even, but not for GELU to 8 bits of a
+    // short shared axis: nothing runs beside its results' work
+    const long wide = tiles(256, 256), rounds = (wide + kUnits - 1) / kUnits;
+    if (k % kBlock == 0 && k >= 2 * kBlock && n % kBlock == 0 && n >= 256 && m >= 256 &&
+        4 * wide >= 3 * rounds * kUnits && !(OUT == kFp8 && a.gelu && k < 2048))
+      return launch_wide<OUT, SF>(a, stream);
+    // 256 x 128 goes round twice a unit at a time: the last round has to be worth it
+    const long large = tiles(256, 128), round = 2 * kUnits;
+    if (large >= 4 * round || 10 * large >= 8 * ((large + round - 1) / round) * round)
+      return launch_tiles<2, 2, 4, 1, OUT, SF>(a, stream);
+  }
+  // exact products too: 256 x 128 has no registers left for their operands. To f32 / to
+  // 8 bits with f32 scales / the same with GELU, beside 8 bits with bf16 scales, us:
+  //   38912 x 3072 x 768      243 / 188 / 240, 100
+  //   103424 x 1024 x 1024    266 / 216 / 260, 113
+  launch_tiles<1, 4, 2, 1, OUT, SF>(a, stream);
+}
+
+}  // namespace
+
+// y in bf16, in f32 where y_f32, or in e4m3 where `ys` takes its scales. Scales, those
+// of y as well, are bf16 or f32 as scales_f32 says.
+void launch_block_gemm(const unsigned char* x, const void* xs, const unsigned char* w,
+                       const void* ws, bool scales_f32, const void* bias, bool bias_f32,
+                       void* y, bool y_f32, void* ys, long x_pitch, long w_pitch, int m,
+                       int n, int k, bool gelu, hipStream_t stream) {
+  const GemmArgs a{x,       w,       xs, ws, bias, y,    ys,
+                   x_pitch, w_pitch, m,  n,  k,    gelu, bias_f32};
+  if (ys)
+    scales_f32 ? launch_best<kFp8, true>(a, stream) : launch_best<kFp8, false>(a, stream);
+  else if (y_f32)
+    scales_f32 ? launch_best<kF32, true>(a, stream) : launch_best<kF32, false>(a, stream);
+  else
+    scales_f32 ? launch_best<kBf16, true>(a, stream) : launch_best<kBf16, false>(a, stream);
 }

@@ -605,7 +605,7 @@ def quantize_fp8_block(
     x: torch.Tensor, scale_dtype: torch.dtype = torch.bfloat16
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """x [..., K] (bf16/f32) -> (x8 [..., K] e4m3, scales [..., ceil(K/128)])."""
-    f32 = _f32_scales("quantize_fp8_block", scale_dtype)
+    f32 = _is_f32("quantize_fp8_block", "scale_dtype", scale_dtype)
     if _serve_hip("quantize_fp8_block", x):
         return _EXT.quantize_fp8_block(x, f32)
     _check_rows("quantize_fp8_block", x)
@@ -617,7 +617,7 @@ def quantize_fp8_block_weight(
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """w [N, K] (bf16/f32) in blocks of 128 x 128 ->
     (w8 [N, K] e4m3, scales [ceil(N/128), ceil(K/128)])."""
-    f32 = _f32_scales("quantize_fp8_block_weight", scale_dtype)
+    f32 = _is_f32("quantize_fp8_block_weight", "scale_dtype", scale_dtype)
     if _serve_hip("quantize_fp8_block_weight", w):
         return _EXT.quantize_fp8_block_weight(w, f32)
     _check_rows("quantize_fp8_block_weight", w)
@@ -641,7 +641,7 @@ def rms_norm_fp8_block(
 ):
     """rms_norm whose y leaves in 8 bits, quantised from its f32 values:
     (y8, scales), and with a residual (y8, scales, x + residual)."""
-    f32 = _f32_scales("rms_norm_fp8_block", scale_dtype)
+    f32 = _is_f32("rms_norm_fp8_block", "scale_dtype", scale_dtype)
     if _serve_hip("rms_norm_fp8_block", x, weight, residual):
         y8, scales, total = _EXT.rms_norm_fp8_block(
             x, residual, weight, eps, f32)
@@ -662,7 +662,7 @@ def layer_norm_fp8_block(
 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """layer_norm(x + residual) in x's dtype and in 8 bits, both from the same
     f32 values: (y, y8, scales). Rows of up to 65536 values."""
-    f32 = _f32_scales("layer_norm_fp8_block", scale_dtype)
+    f32 = _is_f32("layer_norm_fp8_block", "scale_dtype", scale_dtype)
     if _serve_hip("layer_norm_fp8_block", x, weight, bias, residual):
         return _EXT.layer_norm_fp8_block(
             x, residual, weight, bias, eps, f32)
@@ -680,16 +680,20 @@ def fp8_block_linear(
     w_scales: torch.Tensor,
     bias: Optional[torch.Tensor] = None,
     gelu: bool = False,
+    out_dtype: torch.dtype = torch.bfloat16,
 ) -> torch.Tensor:
-    """y [..., N] (bf16) = x @ w.T (+ bias), then exact (erf) GELU if `gelu`, of
+    """y [..., N] (bf16/f32) = x @ w.T (+ bias), then exact (erf) GELU if `gelu`, of
     x8 [..., K] with scales [..., ceil(K/128)] and w8 [N, K] with scales
-    [ceil(N/128), ceil(K/128)]. Accumulated in f32 block by block, rounded
-    once; bias is bf16/f32. Rows at a common distance that is a multiple of
-    16 bytes are read where they lie, others are copied."""
+    [ceil(N/128), ceil(K/128)], both bf16 or both f32. Accumulated in f32 block by
+    block, rounded once; bias is bf16/f32. To bf16 the products within a block are
+    good to some 3e-5 of y (its 2-norm), to f32 they are exact and take twice as long.
+    Rows at a common distance that is a multiple of 16 bytes are read where they lie,
+    others are copied."""
+    f32 = _is_f32("fp8_block_linear", "out_dtype", out_dtype)
     if _serve_hip("fp8_block_linear", x8, x_scales, w8, w_scales, bias):
-        return _EXT.fp8_block_linear(x8, x_scales, w8, w_scales, bias, gelu)
+        return _EXT.fp8_block_linear(x8, x_scales, w8, w_scales, bias, gelu, f32)
     return _block_linear_ref(
-        "fp8_block_linear", x8, x_scales, w8, w_scales, bias, gelu).bfloat16()
+        "fp8_block_linear", x8, x_scales, w8, w_scales, bias, gelu).to(out_dtype)
 
 
 def fp8_block_linear_fp8(
@@ -701,11 +705,12 @@ def fp8_block_linear_fp8(
     gelu: bool = False,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """fp8_block_linear whose y leaves in 8 bits, quantised from its f32
-    values: (y8 [..., N], scales [..., ceil(N/128)])."""
+    values: (y8 [..., N], scales [..., ceil(N/128)] in the type of the others).
+    Where scales are f32 the products are exact, as for an f32 y."""
     if _serve_hip("fp8_block_linear_fp8", x8, x_scales, w8, w_scales, bias):
         return _EXT.fp8_block_linear_fp8(x8, x_scales, w8, w_scales, bias, gelu)
     return _quantize_block_ref(_block_linear_ref(
-        "fp8_block_linear_fp8", x8, x_scales, w8, w_scales, bias, gelu), torch.bfloat16)
+        "fp8_block_linear_fp8", x8, x_scales, w8, w_scales, bias, gelu), x_scales.dtype)
 
 
 # -- the plain forms of the above: the CPU path and the kernels' oracle ------
@@ -740,12 +745,12 @@ def _block_linear_ref(op, x8, x_scales, w8, w_scales, bias, gelu):
     return torch.nn.functional.gelu(y) if gelu else y
 
 
-def _f32_scales(op: str, scale_dtype: torch.dtype) -> bool:
-    if scale_dtype is torch.bfloat16:
+def _is_f32(op: str, name: str, dtype: torch.dtype) -> bool:
+    if dtype is torch.bfloat16:
         return False
-    if scale_dtype is torch.float32:
+    if dtype is torch.float32:
         return True
-    raise RuntimeError(f"{op}: scale_dtype must be bf16/f32, got {scale_dtype}")
+    raise RuntimeError(f"{op}: {name} must be bf16/f32, got {dtype}")
 
 
 def _check_rows(op: str, x: torch.Tensor) -> None:
@@ -780,8 +785,9 @@ def _check_product(op, x8, x_scales, w8, w_scales, bias) -> None:
             raise RuntimeError(f"{op}: arguments on {t.device} and {x8.device}")
     if x8.dtype != torch.float8_e4m3fn or w8.dtype != torch.float8_e4m3fn:
         raise RuntimeError(f"{op}: x8 and w8 must be float8_e4m3fn, got {x8.dtype} and {w8.dtype}")
-    if x_scales.dtype != torch.bfloat16 or w_scales.dtype != torch.bfloat16:
-        raise RuntimeError(f"{op}: scales must be bf16, got {x_scales.dtype} and {w_scales.dtype}")
+    if x_scales.dtype != w_scales.dtype or x_scales.dtype not in (torch.bfloat16, torch.float32):
+        raise RuntimeError(
+            f"{op}: scales must be both bf16 or both f32, got {x_scales.dtype} and {w_scales.dtype}")
     if x8.dim() < 1 or w8.dim() != 2 or x8.shape[-1] != w8.shape[1]:
         raise RuntimeError(
             f"{op}: x8 [..., K] and w8 [N, K] are needed, got {list(x8.shape)} and {list(w8.shape)}")
