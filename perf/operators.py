@@ -241,20 +241,21 @@ def _own(s):
         q, scales = F_ops.fp8_block_linear_fp8(s["x8"], s["xs"], s["w8"], s["ws"], s["b"], gelu=case["gelu"])
         return {"q": q, "scales": scales}
     if op == "ffn":
-        q, scales, total = F_ops.rms_norm_fp8_block(s["x"], s["w"], EPS, residual=s["res"])
+        q, scales, total = F_ops.rms_norm_fp8_block(s["x"], s["w"], EPS, residual=s["res"], scale_dtype=torch.float32)
         q, scales = F_ops.fp8_block_linear_fp8(q, scales, s["w8"], s["ws"], s["b"], gelu=True)
         return {"y": F_ops.fp8_block_linear(q, scales, s["v8"], s["vs"], s["c"]), "sum": total}
     if op == "quant":
-        q, scales = F_ops.quantize_fp8_block(s["x"])
+        q, scales = F_ops.quantize_fp8_block(s["x"], scale_dtype=torch.float32)
         return {"q": q, "scales": scales}
     if op == "quant_weight":
-        q, scales = F_ops.quantize_fp8_block_weight(s["x"])
+        q, scales = F_ops.quantize_fp8_block_weight(s["x"], scale_dtype=torch.float32)
         return {"q": q, "scales": scales}
     if op == "layer8":
-        y, q, scales = F_ops.layer_norm_fp8_block(s["x"], s["w"], s["b"], LN_EPS, residual=s["res"])
+        y, q, scales = F_ops.layer_norm_fp8_block(
+            s["x"], s["w"], s["b"], LN_EPS, residual=s["res"], scale_dtype=torch.float32)
         return {"y": y, "q": q, "scales": scales}
     if op == "rms8":
-        got = F_ops.rms_norm_fp8_block(s["x"], s["w"], EPS, residual=s["res"])
+        got = F_ops.rms_norm_fp8_block(s["x"], s["w"], EPS, residual=s["res"], scale_dtype=torch.float32)
         return dict(zip(("q", "scales", "sum"), got))
     if s["res"] is None:
         y = F_ops.rms_norm(s["x"], s["w"], EPS)
