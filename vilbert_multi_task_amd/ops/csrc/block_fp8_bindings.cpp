@@ -2,8 +2,9 @@
 // norm under torch.ops.vilbert_amd (kernels: block_fp8.hip, block_fp8_gemm.hip).
 
 #include <ATen/ATen.h>
-#include <ATen/hip/EmptyTensor.h>
 #include <ATen/core/DimVector.h>
+#include <ATen/core/dispatch/Dispatcher.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPException.h>
 #include <c10/hip/HIPStream.h>
@@ -134,6 +135,17 @@ void check_norm(const char* op, const at::Tensor& x, const OptTensor& res,
   if (res.has_value()) check_like(op, "residual", x, *res, true);
 }
 
+// Operators by their names: autograd's part of one hands on through the dispatcher, so
+// that what is between it and the kernels (fake tensors, modes, transforms) sees the
+// call. Found once, typed, without boxing.
+#define OPERATOR(name)                                                             \
+  []() -> const auto& {                                                            \
+    static const auto op = c10::Dispatcher::singleton()                            \
+                               .findSchemaOrThrow("vilbert_amd::" #name, "")       \
+                               .typed<decltype(name)>();                           \
+    return op;                                                                     \
+  }()
+
 struct RmsForward {
   at::Tensor y, sum, rstd;  // sum with a residual alone, rstd where asked for
 };
@@ -166,12 +178,27 @@ void rms_bwd_as(const at::Tensor& gy, const OptTensor& gsum,
   C10_HIP_KERNEL_LAUNCH_CHECK();
 }
 
-std::tuple<at::Tensor, at::Tensor> rms_backward(const at::Tensor& gy,
-                                                const OptTensor& gsum,
-                                                const at::Tensor& t,
-                                                const at::Tensor& rstd,
-                                                const at::Tensor& w) {
+// What training takes of the forward: y, the stream (empty without a residual, where
+// it is x) and each row's 1/rms.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_fwd_train(const at::Tensor& x,
+                                                             const OptTensor& res,
+                                                             const at::Tensor& w,
+                                                             double eps) {
+  auto f = rms_forward(x, res, w, eps, true);
+  if (!f.sum.defined()) f.sum = fresh({0}, x.scalar_type(), x);
+  return {f.y, f.sum, f.rstd};
+}
+
+std::tuple<at::Tensor, at::Tensor> rms_bwd(const at::Tensor& gy, const OptTensor& gsum,
+                                           const at::Tensor& t, const at::Tensor& rstd,
+                                           const at::Tensor& w) {
+  const char* op = "rms_bwd";
+  check_norm(op, t, gsum, w);
+  check_like(op, "gy", t, gy, true);
   const long rows = t.numel() / t.size(-1);
+  TORCH_CHECK(rstd.device() == t.device() && rstd.scalar_type() == at::kFloat &&
+                  rstd.dim() == 1 && rstd.size(0) == rows && rstd.is_contiguous(),
+              op, ": rstd must be ", rows, " values in f32 on ", t.device());
   c10::DeviceGuard guard(t.device());
   const auto tc = t.contiguous(), wc = w.contiguous(), gc = gy.contiguous();
   auto gx = fresh_like(tc);
@@ -193,11 +220,11 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
   static List forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x,
                       const at::Tensor& w, const OptTensor& res, double eps) {
     at::AutoDispatchBelowADInplaceOrView below;
-    const auto f = rms_forward(x, res, w, eps, true);
+    const auto [y, sum, rstd] = OPERATOR(rms_fwd_train).call(x, res, w, eps);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({res.has_value() ? f.sum : x, f.rstd, w});
+    ctx->save_for_backward({res.has_value() ? sum : x, rstd, w});
     ctx->saved_data["res"] = res.has_value();
-    return res.has_value() ? List{f.y, f.sum} : List{f.y};
+    return res.has_value() ? List{y, sum} : List{y};
   }
 
   static List backward(torch::autograd::AutogradContext* ctx, List g) {
@@ -208,7 +235,8 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     const at::Tensor gsum = res ? g[1] : at::Tensor();
     at::Tensor gx, gw;
     if (g[0].defined()) {
-      std::tie(gx, gw) = rms_backward(
+      at::AutoDispatchBelowADInplaceOrView below;
+      std::tie(gx, gw) = OPERATOR(rms_bwd).call(
           g[0], gsum.defined() ? OptTensor(gsum) : OptTensor(), saved[0], saved[1],
           saved[2]);
     } else {  // the stream alone was used
@@ -230,7 +258,7 @@ at::Tensor rms_norm(const at::Tensor& x, const at::Tensor& w, double eps) {
 at::Tensor rms_norm_autograd(const at::Tensor& x, const at::Tensor& w, double eps) {
   if (wants_grad(x, {}, w)) return RmsNorm::apply(x, w, OptTensor(), eps)[0];
   at::AutoDispatchBelowADInplaceOrView below;
-  return rms_norm(x, w, eps);
+  return OPERATOR(rms_norm).call(x, w, eps);
 }
 
 std::tuple<at::Tensor, at::Tensor> rms_norm_residual(const at::Tensor& x,
@@ -247,7 +275,7 @@ std::tuple<at::Tensor, at::Tensor> rms_norm_residual_autograd(
     return {y[0], y[1]};
   }
   at::AutoDispatchBelowADInplaceOrView below;
-  return rms_norm_residual(x, res, w, eps);
+  return OPERATOR(rms_norm_residual).call(x, res, w, eps);
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_fp8_block(
@@ -441,22 +469,25 @@ std::tuple<at::Tensor, at::Tensor> fp8_block_linear_fp8(
 }
 
 // The operators without a gradient: what needs one is refused here, for all callers,
-// and the rest goes straight on. (Left to the dispatcher's own fallback, each call
-// would have its arguments boxed.)
+// and the rest is handed on. (The dispatcher's own fallback would box the arguments.)
 bool needs_grad(const at::Tensor& t) { return t.requires_grad(); }
 bool needs_grad(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
 template <typename T>
 bool needs_grad(const T&) { return false; }
 
-template <typename F, F* f, const char* const* name>
+template <typename F, const char* const* name>
 struct Serving;
-template <typename R, typename... A, R (*f)(A...), const char* const* name>
-struct Serving<R(A...), f, name> {
+template <typename R, typename... A, const char* const* name>
+struct Serving<R(A...), name> {
   static R call(A... args) {
-    TORCH_CHECK(!at::GradMode::is_enabled() || !(needs_grad(args) || ...), *name,
+    static const auto op = c10::Dispatcher::singleton()
+                               .findSchemaOrThrow(*name, "")
+                               .typed<R(A...)>();
+    TORCH_CHECK(!at::GradMode::is_enabled() || !(needs_grad(args) || ...),
+                *name + sizeof("vilbert_amd::") - 1,
                 " has no gradient: call it under torch.no_grad()");
     at::AutoDispatchBelowADInplaceOrView below;
-    return f(args...);
+    return op.call(args...);
   }
 };
 
@@ -465,6 +496,8 @@ struct Serving<R(A...), f, name> {
 TORCH_LIBRARY_FRAGMENT(vilbert_amd, m) {
   m.def("rms_norm(Tensor x, Tensor w, float eps) -> Tensor");
   m.def("rms_norm_residual(Tensor x, Tensor res, Tensor w, float eps) -> (Tensor, Tensor)");
+  m.def("rms_fwd_train(Tensor x, Tensor? res, Tensor w, float eps) -> (Tensor, Tensor, Tensor)");
+  m.def("rms_bwd(Tensor gy, Tensor? gsum, Tensor t, Tensor rstd, Tensor w) -> (Tensor, Tensor)");
   m.def("rms_norm_fp8_block(Tensor x, Tensor? res, Tensor w, float eps, bool f32_scales=False) -> (Tensor, Tensor, Tensor)");
   m.def("layer_norm_fp8_block(Tensor x, Tensor? res, Tensor w, Tensor b, float eps, bool f32_scales=False) -> (Tensor, Tensor, Tensor)");
   m.def("quantize_fp8_block(Tensor x, bool f32_scales=False) -> (Tensor, Tensor)");
@@ -476,6 +509,8 @@ TORCH_LIBRARY_FRAGMENT(vilbert_amd, m) {
 TORCH_LIBRARY_IMPL(vilbert_amd, CUDA, m) {
   m.impl("rms_norm", rms_norm);
   m.impl("rms_norm_residual", rms_norm_residual);
+  m.impl("rms_fwd_train", rms_fwd_train);
+  m.impl("rms_bwd", rms_bwd);
   m.impl("rms_norm_fp8_block", rms_norm_fp8_block);
   m.impl("layer_norm_fp8_block", layer_norm_fp8_block);
   m.impl("quantize_fp8_block", quantize_fp8_block);
@@ -487,9 +522,11 @@ TORCH_LIBRARY_IMPL(vilbert_amd, CUDA, m) {
 TORCH_LIBRARY_IMPL(vilbert_amd, AutogradCUDA, m) {
   m.impl("rms_norm", rms_norm_autograd);
   m.impl("rms_norm_residual", rms_norm_residual_autograd);
-#define SERVING(op)                              \
-  static constexpr const char* op##_name = #op; \
-  m.impl(#op, Serving<decltype(op), op, &op##_name>::call)
+#define SERVING(op)                                             \
+  static constexpr const char* op##_name = "vilbert_amd::" #op; \
+  m.impl(#op, Serving<decltype(op), &op##_name>::call)
+  SERVING(rms_fwd_train);
+  SERVING(rms_bwd);
   SERVING(rms_norm_fp8_block);
   SERVING(layer_norm_fp8_block);
   SERVING(quantize_fp8_block);

@@ -620,9 +620,7 @@ def quantize_fp8_block_weight(
     f32 = _is_f32("quantize_fp8_block_weight", "scale_dtype", scale_dtype)
     if _serve_hip("quantize_fp8_block_weight", w):
         return _EXT.quantize_fp8_block_weight(w, f32)
-    _check_rows("quantize_fp8_block_weight", w)
-    if w.dim() != 2:
-        raise RuntimeError(f"quantize_fp8_block_weight: a weight has two dimensions, got {w.dim()}")
+    _check_weight(w)
     n, k = w.shape
     nb, kb = -(-n // FP8_BLOCK), -(-k // FP8_BLOCK)
     v = torch.nn.functional.pad(
@@ -758,6 +756,12 @@ def _check_rows(op: str, x: torch.Tensor) -> None:
         raise RuntimeError(f"{op}: dtype must be bf16/f32, got {x.dtype}")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise RuntimeError(f"{op}: the last dimension is empty")
+
+
+def _check_weight(w: torch.Tensor) -> None:
+    _check_rows("quantize_fp8_block_weight", w)
+    if w.dim() != 2:
+        raise RuntimeError(f"quantize_fp8_block_weight: a weight has two dimensions, got {w.dim()}")
 
 
 def _check_norm(op, x, weight, residual, bias=None) -> None:

@@ -36,6 +36,9 @@ def load():
             f"{path} not built; run `python -m vilbert_multi_task_amd.ops.build`"
         )
     torch.ops.load_library(path)
+    from . import fake
+
+    fake.register()
 
     class _Ext:
         """Proxies every registered vilbert_amd op (no manual listing)."""
