@@ -3,6 +3,7 @@ kernels: fake tensors, dispatch modes, tracing. No kernel may run there."""
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 from torch._subclasses.fake_tensor import FakeTensor, FakeTensorMode
 from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils._python_dispatch import TorchDispatchMode
@@ -134,6 +135,66 @@ def test_refusals_of_fake_tensors():
             F_ops.fp8_block_linear(*p[:3], p[3][:1])
         with pytest.raises(RuntimeError, match="no gradient"):
             F_ops.quantize_fp8_block(x.requires_grad_())
+
+
+def _calls_with_tangents(device):
+    x, w, b, wide, p = _args(device)
+    one = torch.ones_like
+
+    def dual(t):
+        return fwAD.make_dual(t, one(t))
+
+    d, dw = dual(x), dual(w)
+    bias = dual(torch.zeros(130, device=device))
+    return x, d, {
+        "rms_norm_fp8_block": [
+            lambda: F_ops.rms_norm_fp8_block(d, w, EPS), lambda: F_ops.rms_norm_fp8_block(x, dw, EPS),
+            lambda: F_ops.rms_norm_fp8_block(x, w, EPS, residual=d)],
+        "layer_norm_fp8_block": [
+            lambda: F_ops.layer_norm_fp8_block(d, w, b, EPS), lambda: F_ops.layer_norm_fp8_block(x, w, dw, EPS)],
+        "quantize_fp8_block": [lambda: F_ops.quantize_fp8_block(d)],
+        "quantize_fp8_block_weight": [lambda: F_ops.quantize_fp8_block_weight(dual(wide))],
+        "fp8_block_linear": [lambda: F_ops.fp8_block_linear(*p, bias)],
+        "fp8_block_linear_fp8": [
+            lambda: F_ops.fp8_block_linear_fp8(*p, bias),
+            lambda: F_ops.fp8_block_linear_fp8(p[0], dual(p[1]), *p[2:])],
+    }
+
+
+def _refuses_tangents(calls):
+    for name, fs in calls.items():
+        for f in fs:
+            for grad in (True, False):  # no_grad is about the backward pass
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match=name + " has no forward-mode"):
+                    f()
+
+
+def test_tangents_are_refused_not_dropped():
+    with fwAD.dual_level():
+        x, d, calls = _calls_with_tangents("cpu")
+        _refuses_tangents(calls)
+        # the plain norm has its derivative
+        w = torch.ones(200)
+        assert fwAD.unpack_dual(F_ops.rms_norm(d, w, EPS)).tangent is not None
+    with FakeTensorMode(), fwAD.dual_level():
+        x, d, calls = _calls_with_tangents("cuda")
+        _refuses_tangents(calls)
+        w = torch.ones(200, device="cuda")
+        dw = fwAD.make_dual(w, torch.ones_like(w))
+        calls = {"rms_norm": [
+            lambda: F_ops.rms_norm(d, w, EPS), lambda: F_ops.rms_norm(x, dw, EPS),
+            lambda: F_ops.rms_norm(x, w, EPS, residual=d), lambda: F_ops.rms_norm(d, w, EPS, residual=x)]}
+        _refuses_tangents(calls)
+        assert F_ops.rms_norm(x, w, EPS).shape == x.shape  # without one, as ever
+
+
+@gpu
+def test_tangents_are_refused_on_the_gpu():
+    with fwAD.dual_level():
+        x, d, calls = _calls_with_tangents("cuda")
+        w = torch.ones(200, device="cuda")
+        calls["rms_norm"] = [lambda: F_ops.rms_norm(d, w, EPS), lambda: F_ops.rms_norm(x, w, EPS, residual=d)]
+        _refuses_tangents(calls)
 
 
 @gpu

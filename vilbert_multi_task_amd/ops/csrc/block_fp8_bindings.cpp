@@ -5,6 +5,7 @@
 #include <ATen/core/DimVector.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPException.h>
 #include <c10/hip/HIPStream.h>
@@ -246,7 +247,21 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
   }
 };
 
+// No operator here has a forward-mode derivative: left unseen, a tangent would be
+// dropped, and the derivative read as zero.
+bool has_tangent(const at::Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool has_tangent(const OptTensor& t) { return t.has_value() && has_tangent(*t); }
+template <typename T>
+bool has_tangent(const T&) { return false; }
+template <typename... A>
+void refuse_tangents(const char* op, const A&... args) {
+  TORCH_CHECK(!c10::AutogradState::get_tls_state().get_fw_grad_mode() ||
+                  !(has_tangent(args) || ...),
+              op, " has no forward-mode derivative");
+}
+
 bool wants_grad(const at::Tensor& x, const OptTensor& res, const at::Tensor& w) {
+  refuse_tangents("rms_norm", x, res, w);
   return at::GradMode::is_enabled() &&
          (x.requires_grad() || w.requires_grad() ||
           (res.has_value() && res->requires_grad()));
@@ -486,6 +501,7 @@ struct Serving<R(A...), name> {
     TORCH_CHECK(!at::GradMode::is_enabled() || !(needs_grad(args) || ...),
                 *name + sizeof("vilbert_amd::") - 1,
                 " has no gradient: call it under torch.no_grad()");
+    refuse_tangents(*name + sizeof("vilbert_amd::") - 1, args...);
     at::AutoDispatchBelowADInplaceOrView below;
     return op.call(args...);
   }

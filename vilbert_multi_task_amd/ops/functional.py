@@ -23,6 +23,7 @@ import os
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 _EXT = None
 _EXT_ERR: Optional[str] = None
@@ -532,7 +533,7 @@ def rms_norm(
     (y, t) is returned. bf16/f32, rows of up to 65536 values; statistics are
     f32 and y is rounded once. Gradients reach x, weight and residual, once;
     the weight's is added up in a fixed order, so the same inputs give the same
-    bits."""
+    bits. Tensors with a forward-mode tangent are refused on the GPU."""
     if x.is_cuda and not _env_set(b"VILBERT_AMD_FORCE_EAGER") and not (
         _env_set(b"VILBERT_AMD_EAGER_BWD") and torch.is_grad_enabled()
     ):
@@ -578,7 +579,8 @@ def _rms(t, weight, eps):
 # A value that is not finite becomes e4m3's NaN and leaves the block's scale
 # alone. Nothing is kept between calls. On the GPU 8-bit rows begin at
 # multiples of 16 bytes (a view where the width is no such multiple).
-# These are serving operators: inputs that require a gradient are refused.
+# These are serving operators: inputs that require a gradient or have a
+# forward-mode tangent are refused.
 # --------------------------------------------------------------------------
 
 FP8_BLOCK = 128
@@ -587,8 +589,8 @@ _SCALE_MIN = 2.0 ** -100
 
 
 def _serve_hip(op: str, *tensors: Optional[torch.Tensor]) -> bool:
-    """True iff the HIP path should run; what needs a gradient is refused, here or
-    there."""
+    """True iff the HIP path should run; what needs a gradient, or carries a
+    forward-mode tangent, is refused, here or there."""
     if tensors[0].is_cuda and not _env_set(b"VILBERT_AMD_FORCE_EAGER"):
         if _EXT is None:
             _require_extension()
@@ -598,6 +600,9 @@ def _serve_hip(op: str, *tensors: Optional[torch.Tensor]) -> bool:
             if t is not None and t.requires_grad:
                 raise RuntimeError(
                     f"{op} has no gradient: call it under torch.no_grad()")
+    for t in tensors:
+        if t is not None and unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{op} has no forward-mode derivative")
     return False
 
 
