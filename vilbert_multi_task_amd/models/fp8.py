@@ -167,8 +167,16 @@ def attach_quant_pack(x: torch.Tensor, ctx: Fp8Context, site: int) -> torch.Tens
     return x
 
 
+def _refuse_converted(bert) -> None:
+    """A conversion is of the whole encoder or of nothing."""
+    for m in bert.modules():
+        if isinstance(m, (Fp8Linear, BlockFp8Linear)):
+            raise RuntimeError("the encoder's products are in 8 bits already")
+
+
 def convert_encoder_to_fp8(model) -> int:
-    """Swap the two-stream encoder onto the fp8 path. Returns #GEMM sites."""
+    """Swap the two-stream encoder onto the fp8 path. Returns #GEMM sites.
+    One that is in 8 bits already, in either way, is refused."""
     from .vilbert import (
         CrossAttention,
         FeedForward,
@@ -178,6 +186,7 @@ def convert_encoder_to_fp8(model) -> int:
     )
 
     bert = model.bert if hasattr(model, "bert") else model
+    _refuse_converted(bert)
     device = next(bert.parameters()).device
 
     # pass 1: count quantization sites
@@ -310,7 +319,8 @@ class BlockFp8LayerNorm(nn.Module):
 
 def convert_encoder_to_fp8_block(model) -> int:
     """Swap the two-stream encoder's products onto e4m3 with a scale per block
-    of 128. For inference (no gradient). Returns #GEMM sites."""
+    of 128. For inference (no gradient). Returns #GEMM sites. One that is in 8 bits
+    already, in either way, is refused."""
     from ..ops import functional as F_ops
     from .vilbert import (
         CrossAttention,
@@ -321,9 +331,7 @@ def convert_encoder_to_fp8_block(model) -> int:
     )
 
     bert = model.bert if hasattr(model, "bert") else model
-    for m in bert.modules():  # as a whole or not at all
-        if isinstance(m, (Fp8Linear, BlockFp8Linear)):
-            raise RuntimeError("the encoder's products are in 8 bits already")
+    _refuse_converted(bert)
     n_gemms = 0
     with torch.no_grad():
         for m in list(bert.modules()):
