@@ -6,6 +6,7 @@ import torch
 from vilbert_multi_task_amd.config import ViLBertConfig
 from vilbert_multi_task_amd.models import VILBertForVLTasks
 from vilbert_multi_task_amd.models.fp8 import (
+    BlockFp8Linear,
     convert_encoder_to_fp8,
     convert_encoder_to_fp8_block,
 )
@@ -32,3 +33,61 @@ def test_a_second_conversion_is_refused_and_changes_nothing(first, second):
     for (name, key), (t, before) in held.items():
         assert getattr(parts[name], key) is t
         assert torch.equal(t.float(), before.float())
+
+
+def _linears(model):
+    return [m for m in model.modules() if isinstance(m, BlockFp8Linear)]
+
+
+@pytest.mark.parametrize("cast", [
+    lambda m: m.to(torch.bfloat16), lambda m: m.bfloat16(), lambda m: m.half(), lambda m: m.double(),
+    lambda m: m.to("cpu"), lambda m: m.to(torch.bfloat16).float()])
+def test_casts_leave_8_bit_weights_and_their_scales(cast):
+    model = _model()
+    convert_encoder_to_fp8_block(model)
+    before = [(m.w8.clone(), m.w_scales.clone()) for m in _linears(model)]
+    cast(model)
+    assert before
+    for m, (w8, scales) in zip(_linears(model), before):
+        assert m.w8.dtype == torch.float8_e4m3fn and m.w_scales.dtype == torch.bfloat16
+        assert torch.equal(m.w8.float(), w8.float()) and torch.equal(m.w_scales, scales)
+        assert {"w8", "w_scales", "bias"} == set(m.state_dict())
+
+
+def test_a_cast_module_answers_in_its_new_type():
+    torch.manual_seed(1)
+    for bias in (True, False):
+        m = BlockFp8Linear(torch.nn.Linear(96, 200, bias=bias))
+        x = torch.randn(5, 96)
+        want = m(x)
+        assert want.dtype == torch.float32
+        q, s = m.to(torch.bfloat16).gelu8(x.bfloat16())
+        assert m(x.bfloat16()).dtype == torch.bfloat16
+        wide = BlockFp8Linear(torch.nn.Linear(200, 8)).to(torch.bfloat16)
+        assert wide((q, s)).dtype == torch.bfloat16  # a pair has no type of its own
+        assert torch.equal(m.float()(x), want) or bias  # a bias was rounded on the way
+
+
+def test_a_state_dict_is_taken_up_again():
+    a, b = _model(), _model()
+    convert_encoder_to_fp8_block(a)
+    with torch.no_grad():
+        for p in b.parameters():
+            p.mul_(1.5)
+    convert_encoder_to_fp8_block(b)
+    b.load_state_dict(a.state_dict())
+    for m, n in zip(_linears(a), _linears(b)):
+        assert torch.equal(m.w8.float(), n.w8.float()) and torch.equal(m.w_scales, n.w_scales)
+
+
+@pytest.mark.gpu
+def test_a_module_moves_to_the_gpu_as_it_is():
+    torch.manual_seed(1)
+    m = BlockFp8Linear(torch.nn.Linear(100, 60))  # rows that are no multiple of 16 bytes
+    x = torch.randn(7, 100)
+    want = m(x)
+    got = m.cuda()(x.cuda())
+    assert got.dtype == want.dtype
+    # both round once to bf16; the 8-bit instruction drops 2^-13 of the largest of eight
+    # products for 7 of them, of sizes that add up to about 4
+    assert torch.allclose(got.cpu(), want, rtol=2.0 ** -7, atol=7 * 2.0 ** -13 * 4)

@@ -283,7 +283,26 @@ class BlockFp8Linear(nn.Module):
             "bias", None if linear.bias is None else linear.bias.detach())
         self.in_features = linear.in_features
         self.out_features = linear.out_features
-        self.dtype = linear.weight.dtype
+        # of no size: what type the module's results have, also after a cast
+        self.register_buffer("_like", linear.weight.detach().new_empty(0), persistent=False)
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return self._like.dtype
+
+    def _apply(self, fn, recurse=True):
+        """Moves the 8-bit weight and its scales with the rest, and casts neither:
+        what moves them sees whole numbers."""
+        held = {}
+        for name, as_int in (("w8", torch.uint8), ("w_scales", torch.int16)):
+            t = self._buffers[name]
+            held[name] = fn(t.view(as_int)).view(t.dtype)
+        for name in held:
+            del self._buffers[name]
+        try:
+            return super()._apply(fn, recurse)
+        finally:
+            self._buffers.update(held)
 
     def forward(self, x) -> torch.Tensor:
         return fp8_block_mm(x, self.w8, self.w_scales, self.bias).to(self.dtype)
