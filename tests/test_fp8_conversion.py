@@ -6,10 +6,13 @@ import torch
 from vilbert_multi_task_amd.config import ViLBertConfig
 from vilbert_multi_task_amd.models import VILBertForVLTasks
 from vilbert_multi_task_amd.models.fp8 import (
+    BlockFp8LayerNorm,
     BlockFp8Linear,
+    _block_pack,
     convert_encoder_to_fp8,
     convert_encoder_to_fp8_block,
 )
+from vilbert_multi_task_amd.models.vilbert import FusedLayerNorm
 
 
 def _model():
@@ -91,3 +94,33 @@ def test_a_module_moves_to_the_gpu_as_it_is():
     # both round once to bf16; the 8-bit instruction drops 2^-13 of the largest of eight
     # products for 7 of them, of sizes that add up to about 4
     assert torch.allclose(got.cpu(), want, rtol=2.0 ** -7, atol=7 * 2.0 ** -13 * 4)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_what_is_written_over_is_quantised_anew(device):
+    """The norm's 8-bit form stands for the values that it was made with alone."""
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    torch.manual_seed(1)
+    norm = BlockFp8LayerNorm(FusedLayerNorm(96, 1e-5)).to(device, dtype)
+    linear = BlockFp8Linear(torch.nn.Linear(96, 40).to(device, dtype))
+    x = torch.randn(5, 96, device=device, dtype=dtype)
+    change = [
+        lambda y: y.mul_(3), lambda y: y[1:].zero_(), lambda y: y.copy_(x), lambda y: y.view(-1)[7:9].fill_(50)]
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            for f in change:
+                y = norm(x)
+                f(y)
+                assert torch.equal(linear(y), linear(y.clone()))
+                q, s = linear.gelu8(y)
+                rq, rs = linear.gelu8(y.clone())
+                assert torch.equal(q.float(), rq.float()) and torch.equal(s, rs)
+
+
+def test_the_norms_8_bit_form_is_what_is_used():
+    norm = BlockFp8LayerNorm(FusedLayerNorm(96, 1e-5))
+    linear = BlockFp8Linear(torch.nn.Linear(96, 40))
+    with torch.no_grad():
+        y = norm(torch.randn(5, 96))
+        assert _block_pack(y)[0] is y._fp8b[0] and _block_pack(y)[1] is y._fp8b[1]
+        linear(y)

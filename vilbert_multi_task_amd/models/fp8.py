@@ -246,15 +246,15 @@ def convert_encoder_to_fp8(model) -> int:
 
 def _block_pack(x):
     """x in 8 bits: as it is where it is (values, scales) already, what its
-    producer emitted, or quantised here."""
+    producer emitted where x has not been written since, or quantised here."""
     if isinstance(x, tuple):
         return x
     pack = getattr(x, "_fp8b", None)
-    if pack is None:
-        from ..ops import functional as F_ops
+    if pack is not None and pack[2] == x._version:
+        return pack[:2]
+    from ..ops import functional as F_ops
 
-        pack = F_ops.quantize_fp8_block(x)
-    return pack
+    return F_ops.quantize_fp8_block(x)
 
 
 def fp8_block_mm(
@@ -317,7 +317,8 @@ class BlockFp8Linear(nn.Module):
 
 
 class BlockFp8LayerNorm(nn.Module):
-    """FusedLayerNorm replacement that emits the 8-bit form as well (`_fp8b`)."""
+    """FusedLayerNorm replacement that emits the 8-bit form as well (`_fp8b`: values,
+    scales and the version of the result that they belong to)."""
 
     def __init__(self, ln):
         super().__init__()
@@ -332,7 +333,8 @@ class BlockFp8LayerNorm(nn.Module):
             return F_ops.layer_norm(x, self.weight, self.bias, self.eps, residual)
         y, y8, scales = F_ops.layer_norm_fp8_block(
             x, self.weight, self.bias, self.eps, residual=residual)
-        y._fp8b = (y8, scales)
+        if not y.is_inference():  # those do not count their writes
+            y._fp8b = (y8, scales, y._version)
         return y
 
 
