@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from vilbert_multi_task_amd.config import ViLBertConfig
+from vilbert_multi_task_amd.engine.runner import GraphRunner
 from vilbert_multi_task_amd.models import VILBertForVLTasks
 from vilbert_multi_task_amd.models.fp8 import (
     BlockFp8LayerNorm,
@@ -124,3 +125,14 @@ def test_the_norms_8_bit_form_is_what_is_used():
         y = norm(torch.randn(5, 96))
         assert _block_pack(y)[0] is y._fp8b[0] and _block_pack(y)[1] is y._fp8b[1]
         linear(y)
+
+
+@pytest.mark.parametrize("fp8", [None, False, 0, "", True, 1, "block"])
+def test_runner_takes_what_says_yes_or_no(fp8):
+    GraphRunner(_model(), device="cpu", fp8=fp8)
+
+
+@pytest.mark.parametrize("fp8", ["tensor", "blocks", 2, object()])
+def test_runner_refuses_other_modes(fp8):
+    with pytest.raises(ValueError, match="fp8"):
+        GraphRunner(_model(), device="cpu", fp8=fp8)

@@ -32,7 +32,7 @@ class GraphRunner:
         serving_fast: bool = False,
         fp8: Union[bool, str] = False,  # True: a scale per tensor; "block": per 128 values
     ):
-        if fp8 not in (False, True, "block"):
+        if fp8 and fp8 not in (True, "block"):
             raise ValueError(f"fp8 must be False, True or 'block', got {fp8!r}")
         self.model = model.eval()
         if hasattr(model, "prepare_for_serving"):
