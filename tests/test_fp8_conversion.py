@@ -1,5 +1,9 @@
 """Converting an encoder to 8-bit products: once, as a whole, and what it keeps after."""
 
+import argparse
+import dataclasses
+import json
+
 import pytest
 import torch
 
@@ -14,6 +18,7 @@ from vilbert_multi_task_amd.models.fp8 import (
     convert_encoder_to_fp8_block,
 )
 from vilbert_multi_task_amd.models.vilbert import FusedLayerNorm
+from vilbert_multi_task_amd.serve.main import build_worker
 
 
 def _model():
@@ -136,3 +141,15 @@ def test_runner_takes_what_says_yes_or_no(fp8):
 def test_runner_refuses_other_modes(fp8):
     with pytest.raises(ValueError, match="fp8"):
         GraphRunner(_model(), device="cpu", fp8=fp8)
+
+
+@pytest.mark.parametrize("more", [{}, {"fp8_block": True}])
+def test_a_worker_is_built_with_and_without_the_mode(more, tmp_path):
+    """Callers that were there before the mode say nothing of it."""
+    config = tmp_path / "tiny.json"
+    config.write_text(json.dumps(dataclasses.asdict(ViLBertConfig.tiny())))
+    args = argparse.Namespace(
+        config=str(config), checkpoint="", device=-1, fp8=False, detector=False,
+        queue=str(tmp_path / "q"), db=str(tmp_path / "d"), hub_port=0, vqa_answers="", gqa_answers="",
+        max_batch=4, **more)
+    assert build_worker(args).runner is not None

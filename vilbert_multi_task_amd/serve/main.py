@@ -67,8 +67,9 @@ def build_worker(args):
     if device.startswith("cuda"):
         model = model.to(device=device, dtype=torch.bfloat16)
     runner = GraphRunner(
-        model, device=device, use_graphs=device.startswith("cuda"),
-        serving_fast=True, fp8="block" if args.fp8_block else args.fp8, feat_dim=cfg.v_feature_size,
+        model, device=device, use_graphs=device.startswith("cuda"), serving_fast=True,
+        fp8="block" if getattr(args, "fp8_block", False) else args.fp8,
+        feat_dim=cfg.v_feature_size,
     )
 
     provider = None
