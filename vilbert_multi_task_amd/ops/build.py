@@ -14,6 +14,7 @@ import os
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
+from typing import List
 
 import torch
 import torch.utils.cpp_extension as ce
@@ -37,24 +38,31 @@ def _mtime(path: str) -> float:
 
 
 def _src_mtime(source: str) -> float:
-    return max(_mtime(os.path.join(CSRC, s)) for s in [source] + HEADERS)
+    return max(os.path.getmtime(os.path.join(CSRC, s)) for s in [source] + HEADERS)
 
 
-def needs_build() -> bool:
-    return _mtime(OUT_SO) < max(_src_mtime(s) for s in SOURCES)
+def _object(source: str) -> str:
+    return os.path.join(OBJ_DIR, source + ".o")
 
 
-def build(force: bool = False, verbose: bool = True, asan: bool = False,
-          ubsan: bool = False) -> str:
-    """Compile what is older than its source (``force``: everything), one
-    object per source and several at a time, and link."""
-    if not force and not needs_build():
-        return OUT_SO
-    os.makedirs(OBJ_DIR, exist_ok=True)
-    hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    torch_lib = ce.library_paths()[0]
-    abi = int(torch.compiled_with_cxx11_abi())
-    flags = [
+def _sanitize(asan: bool, ubsan: bool) -> List[str]:
+    if ubsan:
+        # UndefinedBehaviorSanitizer, host side: no allocator interception,
+        # coexists with the HIP runtime (ASan's interceptors do not)
+        return ["-Xarch_host", "-fsanitize=undefined",
+                "-Xarch_host", "-fno-sanitize=vptr,function",
+                "-Xarch_host", "-fno-sanitize-recover=undefined",
+                "-shared-libsan", "-g1"]
+    if asan:
+        # host-side AddressSanitizer (scripts/sanitize.sh); device code is
+        # not instrumented
+        return ["-Xarch_host", "-fsanitize=address", "-shared-libsan", "-g1"]
+    return []
+
+
+def _compile_command(source: str, sanitize: List[str]) -> List[str]:
+    return [
+        os.environ.get("HIPCC", "/opt/rocm/bin/hipcc"),
         f"--offload-arch={ARCH}",
         "-O3",
         "-std=c++17",
@@ -62,40 +70,22 @@ def build(force: bool = False, verbose: bool = True, asan: bool = False,
         "-fno-gpu-rdc",
         # some forms of the packed f32 instructions have given wrong results
         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-        f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
         "-DUSE_ROCM",
         "-D__HIP_PLATFORM_AMD__",
         "-DTORCH_EXTENSION_NAME=vilbert_hip",
+        *sanitize,
+        *(f"-I{inc}" for inc in ce.include_paths()),
+        "-c", os.path.join(CSRC, source),
     ]
-    sanitize = []
-    if asan:
-        # host-side AddressSanitizer (scripts/sanitize.sh); device code is
-        # not instrumented
-        sanitize = ["-Xarch_host", "-fsanitize=address", "-shared-libsan", "-g1"]
-    if ubsan:
-        # UndefinedBehaviorSanitizer, host side: no allocator interception,
-        # coexists with the HIP runtime (ASan's interceptors do not)
-        sanitize = ["-Xarch_host", "-fsanitize=undefined",
-                    "-Xarch_host", "-fno-sanitize=vptr,function",
-                    "-Xarch_host", "-fno-sanitize-recover=undefined",
-                    "-shared-libsan", "-g1"]
-    incs = [f"-I{inc}" for inc in ce.include_paths()]
 
-    def compile_one(source: str) -> str:
-        src = os.path.join(CSRC, source)
-        obj = os.path.join(OBJ_DIR, source + ".o")
-        if force or _mtime(obj) < _src_mtime(source):
-            cmd = [hipcc, *flags, *sanitize, *incs, "-c", src, "-o", obj]
-            if verbose:
-                print("[vilbert_amd.ops.build]", " ".join(cmd), flush=True)
-            subprocess.run(cmd, check=True)
-        return obj
 
-    jobs = min(int(os.environ.get("MAX_JOBS", "8")), os.cpu_count() or 1, 16)
-    with ThreadPoolExecutor(max_workers=jobs) as pool:
-        objs = list(pool.map(compile_one, SOURCES))
-    link = [
-        hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *sanitize, *objs,
+def _link_command(sanitize: List[str]) -> List[str]:
+    torch_lib = ce.library_paths()[0]
+    return [
+        os.environ.get("HIPCC", "/opt/rocm/bin/hipcc"),
+        f"--offload-arch={ARCH}", "-shared", "-fPIC", *sanitize,
+        *(_object(s) for s in SOURCES),
         f"-L{torch_lib}",
         f"-Wl,-rpath,{torch_lib}",
         "-ltorch",
@@ -105,12 +95,67 @@ def build(force: bool = False, verbose: bool = True, asan: bool = False,
         "-lc10_hip",
         "-lamdhip64",
         "-lhipblaslt",
-        "-o",
-        OUT_SO,
     ]
+
+
+# Beside what is built lies how it was: a file is used again only where it is newer than
+# its sources and would be made by the same commands, under the same torch.
+def _made_by(*commands: List[str]) -> str:
+    return "\n".join([torch.__version__, *(" ".join(c) for c in commands)])
+
+
+def _is_made_by(path: str, made_by: str) -> bool:
+    try:
+        with open(path + ".made_by") as f:
+            return os.path.exists(path) and f.read() == made_by
+    except OSError:
+        return False
+
+
+def _make(path: str, command: List[str], made_by: str, verbose: bool) -> None:
+    """Whole or not at all: the file is put in its place when it is done."""
+    part = f"{path}.{os.getpid()}.part"
     if verbose:
-        print("[vilbert_amd.ops.build]", " ".join(link), flush=True)
-    subprocess.run(link, check=True)
+        print("[vilbert_amd.ops.build]", " ".join(command), "-o", path, flush=True)
+    try:
+        subprocess.run([*command, "-o", part], check=True)
+        if os.path.exists(path + ".made_by"):
+            os.remove(path + ".made_by")
+        os.replace(part, path)
+    finally:
+        if os.path.exists(part):
+            os.remove(part)
+    with open(path + ".made_by", "w") as f:
+        f.write(made_by)
+
+
+def needs_build(asan: bool = False, ubsan: bool = False) -> bool:
+    sanitize = _sanitize(asan, ubsan)
+    made_by = _made_by(*(_compile_command(s, sanitize) for s in SOURCES), _link_command(sanitize))
+    return not _is_made_by(OUT_SO, made_by) or _mtime(OUT_SO) < max(_src_mtime(s) for s in SOURCES)
+
+
+def build(force: bool = False, verbose: bool = True, asan: bool = False,
+          ubsan: bool = False) -> str:
+    """Compile what is older than its source or was compiled in another way
+    (``force``: everything), one object per source and several at a time, and link."""
+    if not force and not needs_build(asan, ubsan):
+        return OUT_SO
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    sanitize = _sanitize(asan, ubsan)
+
+    def compile_one(source: str) -> List[str]:
+        obj, command = _object(source), _compile_command(source, sanitize)
+        made_by = _made_by(command)
+        if force or not _is_made_by(obj, made_by) or _mtime(obj) < _src_mtime(source):
+            _make(obj, command, made_by, verbose)
+        return command
+
+    jobs = max(1, min(int(os.environ.get("MAX_JOBS") or 8), os.cpu_count() or 1, 16))
+    with ThreadPoolExecutor(max_workers=jobs) as pool:
+        commands = list(pool.map(compile_one, SOURCES))
+    link = _link_command(sanitize)
+    _make(OUT_SO, link, _made_by(*commands, link), verbose)
     return OUT_SO
 
 
