@@ -1,6 +1,9 @@
 """The block-scaled operators and the rms norm seen from between autograd and the
 kernels: fake tensors, dispatch modes, tracing. No kernel may run there."""
 
+import collections.abc
+import os
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
@@ -248,3 +251,46 @@ def test_backward_operator_checks_what_it_is_given():
     ):
         with pytest.raises(RuntimeError, match="rms_bwd"):
             ext.rms_bwd(*bad)
+
+
+class _Environ(collections.abc.MutableMapping):
+    """An environment by its public interface alone."""
+
+    def __init__(self, values):
+        self._values = dict(values)
+
+    def __getitem__(self, name):
+        return self._values[name]
+
+    def __setitem__(self, name, value):
+        self._values[name] = value
+
+    def __delitem__(self, name):
+        del self._values[name]
+
+    def __iter__(self):
+        return iter(self._values)
+
+    def __len__(self):
+        return len(self._values)
+
+
+def test_switches_are_read_as_they_are_at_the_call(monkeypatch):
+    env = _Environ(os.environ)
+    monkeypatch.setattr(os, "environ", env)
+    with FakeTensorMode(), torch.no_grad(), _Seen() as seen:
+        x, w, b, wide, p = _args("cuda")
+        for name, op, call in (
+            ("VILBERT_AMD_FORCE_EAGER", "rms_norm", lambda: F_ops.rms_norm(x, w, EPS)),
+            ("VILBERT_AMD_FORCE_EAGER", "quantize_fp8_block", lambda: F_ops.quantize_fp8_block(x)),
+            ("VILBERT_AMD_FORCE_EAGER", "fp8_block_linear", lambda: F_ops.fp8_block_linear(*p)),
+            ("VILBERT_AMD_EAGER_BWD", "rms_norm", lambda: torch.enable_grad()(F_ops.rms_norm)(x, w, EPS)),
+        ):
+            for value, own in ((None, True), ("1", False), ("0", True)):
+                env.pop(name, None)
+                if value is not None:
+                    env[name] = value
+                seen.names.clear()
+                call()
+                assert ("vilbert_amd::" + op in seen.names) == own, (name, value, op)
+            env.pop(name)

@@ -534,8 +534,8 @@ def rms_norm(
     f32 and y is rounded once. Gradients reach x, weight and residual, once;
     the weight's is added up in a fixed order, so the same inputs give the same
     bits. Tensors with a forward-mode tangent are refused on the GPU."""
-    if x.is_cuda and not _env_set(b"VILBERT_AMD_FORCE_EAGER") and not (
-        _env_set(b"VILBERT_AMD_EAGER_BWD") and torch.is_grad_enabled()
+    if x.is_cuda and os.environ.get("VILBERT_AMD_FORCE_EAGER") != "1" and not (
+        torch.is_grad_enabled() and os.environ.get("VILBERT_AMD_EAGER_BWD") == "1"
     ):
         ext = _EXT or _require_extension()
         if residual is None:
@@ -545,15 +545,6 @@ def rms_norm(
     t = x if residual is None else x + residual
     y = _rms(t, weight, eps).to(x.dtype)
     return y if residual is None else (y, t)
-
-
-# os.environ.get takes a microsecond for a name that is not set, an eighth of a small
-# call: an exception inside. What it holds is a dict of bytes, asked as it is.
-_ENV = os.environ._data
-
-
-def _env_set(name: bytes) -> bool:
-    return _ENV.get(name) == b"1"
 
 
 def _require_extension():
@@ -591,7 +582,7 @@ _SCALE_MIN = 2.0 ** -100
 def _serve_hip(op: str, *tensors: Optional[torch.Tensor]) -> bool:
     """True iff the HIP path should run; what needs a gradient, or carries a
     forward-mode tangent, is refused, here or there."""
-    if tensors[0].is_cuda and not _env_set(b"VILBERT_AMD_FORCE_EAGER"):
+    if tensors[0].is_cuda and os.environ.get("VILBERT_AMD_FORCE_EAGER") != "1":
         if _EXT is None:
             _require_extension()
         return True
