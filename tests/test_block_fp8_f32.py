@@ -358,3 +358,30 @@ def test_exact_outputs_past_32_bits():
     del y
     q, s = F_ops.fp8_block_linear_fp8(big.view(E4), scales, w8, ws)
     _check_rows(q[-4:], s[-4:], y64, off)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("m,n,k", [(5, 128, 128), (40, 300, 300), (600, 1030, 300), (2500, 1000, 128), (4100, 1030, 300), (16300, 1024, 384)])
+def test_scales_whose_product_passes_the_range(m, n, k, device):
+    """What is nothing stays nothing, however large the scales beside it are."""
+    if device == "cpu":
+        m = 5
+    x8, xs, w8, ws = _operands(m, n, k, device)
+    b = _normal(n, seed=5).to(device)
+    cases = [(BF, BF), (BF, F32), (F32, BF), (F32, F32)]  # scales, results
+    want = [F_ops.fp8_block_linear(x8, xs.to(s), w8, ws.to(s), b, out_dtype=o) for s, o in cases]
+    x8.view(torch.uint8)[3] = 0
+    xs[3], ws[0] = 6e35, 1000.0
+    xs[1], ws[-1, -1] = 2.0 ** -100, 2.0 ** -100
+    small = x8.view(torch.uint8).clone()
+    small[1, k // 128 * 128 if k % 128 else k - 128:] = 0  # and where a product is 2^-200
+    x8 = small.view(E4)
+    for (s, o), ref in zip(cases, want):
+        y = F_ops.fp8_block_linear(x8, xs.to(s), w8, ws.to(s), b, out_dtype=o)
+        assert torch.equal(y[3], b.to(o))
+        # rows of ordinary scales are what they were, where W's are
+        at = slice(128, (n - 1) // 128 * 128)
+        assert torch.equal(y[4, at], ref[4, at]) and not torch.isnan(y).any()
+    xs[3, 0] = math.nan  # a scale that is none is not hidden
+    assert torch.isnan(F_ops.fp8_block_linear(x8, xs, w8, ws, b)[3]).all()
+    assert torch.isnan(F_ops.fp8_block_linear(x8, xs, w8, ws, b, out_dtype=F32)[3]).all()

@@ -63,6 +63,11 @@ template <bool SF>
 DEV float scale_value(unsigned held) {
   return SF ? __uint_as_float(held) : us2f((unsigned short)held);
 }
+// The scale of a block's products. Where two scales' product passes f32's range it is
+// f32's largest number, not infinity, which times a block sum of nothing would be NaN.
+DEV float both_scales(float x, float w) {
+  return __builtin_elementwise_minimum(x * w, 3.40282347e38f);
+}
 
 // What leaves in 32 bits has to be right in 32.
 template <Out OUT, bool SF>
@@ -241,7 +246,7 @@ __global__ __launch_bounds__(512) void block_gemm_direct_kernel(GemmArgs a) {
     for (int u = 0; u < MT; ++u) x[u] = load32_row(xrow[u], k, a.k);
     const float wsb = scale_value<SF>(ws[b]);
 #pragma unroll
-    for (int u = 0; u < MT; ++u) s[u] = scale_value<SF>(xs[u][b]) * wsb;
+    for (int u = 0; u < MT; ++u) s[u] = both_scales(scale_value<SF>(xs[u][b]), wsb);
   };
   f32x4 acc[NT][MT] = {};
   if (kw < kb) load(kw);
@@ -452,7 +457,8 @@ block_gemm_tile_kernel(GemmArgs a, int mtiles, int ntiles) {
     const float w = scale_value<SF>(__builtin_amdgcn_readlane(ws4, from));
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      s[t] = w * scale_value<SF>(__builtin_amdgcn_ds_bpermute((from + r) * 4, xs4[t]));
+      s[t] = both_scales(
+          scale_value<SF>(__builtin_amdgcn_ds_bpermute((from + r) * 4, xs4[t])), w);
       // here and not later, where waiting for them would be waiting for W
       asm volatile("" : "+v"(s[t]));
     }
@@ -827,7 +833,7 @@ __global__ __launch_bounds__(512, 2) void block_gemm_wide_kernel(GemmArgs a, int
   auto take_scales = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      s[u] = scale_value<SF>(raw[4]) * scale_value<SF>(raw[u]);
+      s[u] = both_scales(scale_value<SF>(raw[u]), scale_value<SF>(raw[4]));
   };
 
   enter();

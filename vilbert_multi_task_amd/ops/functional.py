@@ -681,6 +681,8 @@ def fp8_block_linear(
     [ceil(N/128), ceil(K/128)], both bf16 or both f32. Accumulated in f32 block by
     block, rounded once; bias is bf16/f32. To bf16 the products within a block are
     good to some 3e-5 of y (its 2-norm), to f32 they are exact and take twice as long.
+    The product of two scales is one of f32's normal numbers: on the GPU a larger one is
+    taken as the largest of them, a smaller one may be taken as 0.
     Rows at a common distance that is a multiple of 16 bytes are read where they lie,
     others are copied."""
     f32 = _is_f32("fp8_block_linear", "out_dtype", out_dtype)
