@@ -1015,19 +1015,36 @@ void launch_direct(const GemmArgs& a, hipStream_t stream) {
 //   6464 x 3072 x 768                                      36      28       24       26
 //   16384 x 1024 x 1024                                            27       30       23
 //   103424 x 1024 x 1024                                          157      139      128
+// That is one call over and over, its operands in the caches. Of few rows what counts
+// is where W comes from; with other weights each call (60 MB of them), as in a model:
+//   38 x 8192 x 4096               29     18               21      28
+//   256 x 1601 x 1024              11      7.7              9.1    10.3
+//   608 x 768 x 1024               10      6.7              8.4     9.4
+//   608 x 768 x 3072               23     13.8             16.8    20.6
+//   1024 x 512 x 4096              32     18.6             20.1    25.8
+// so that the direct kernel has them, also where two teams are faster in a loop.
 //
 // Tiles of 256 x 256 in turn with the best of the others; rounds of 256 tiles, to
-// bf16 / to bf16 with GELU / to 8 bits / to 8 bits with GELU:
-//   rows x width x shared   rounds  others                      256 x 256
-//   9728 x 768 x 3072        0.45    34.0 / 35.6 / 32.5 / 34.1   39.9 / 43.4 / 38.0 / 42.3
-//   12928 x 1024 x 1024      0.80    24.7 / 28.6 / 24.2 / 28.2   20.7 / 24.6 / 19.1 / 24.1
-//   6464 x 3072 x 768        1.22    25.3 / 29.9 / 23.4 / 28.5   29.6 / 37.2 / 27.5 / 38.0
-//   9728 x 3072 x 768        1.78    35.3 / 43.2 / 32.1 / 39.2   33.8 / 39.9 / 29.0 / 39.3
-//   38912 x 768 x 3072       1.78    106 / 102 / 88.0 / 93.3     95.1 / 89.9 / 77.8 / 87.1
-//   103424 x 1024 x 1024     6.31    136 / 146 / 110 / 130       128 / 140 / 105 / 138
-//   38912 x 3072 x 768       7.13    124 / 141 / 100 / 124       116 / 138 / 96.5 / 134
-//   38912 x 3072 x 1536      7.13    204 / 214 / 178 / 201       186 / 201 / 167 / 205
-//   16384 x 4096 x 4096      4.00    272 / 263 / 245 / 255       231 / 232 / 213 / 237
+// bf16 / to bf16 with GELU / to 8 bits, one call over and over:
+//   rows x width x shared   rounds  others                256 x 256
+//   9728 x 768 x 3072        0.45    34.0 / 35.6 / 32.5    39.9 / 43.4 / 38.0
+//   12928 x 1024 x 1024      0.80    24.7 / 28.6 / 24.2    20.7 / 24.6 / 19.1
+//   6464 x 3072 x 768        1.22    25.3 / 29.9 / 23.4    29.6 / 37.2 / 27.5
+//   9728 x 3072 x 768        1.78    35.3 / 43.2 / 32.1    33.8 / 39.9 / 29.0
+//   38912 x 768 x 3072       1.78    106 / 102 / 88.0      95.1 / 89.9 / 77.8
+//   103424 x 1024 x 1024     6.31    136 / 146 / 110       128 / 140 / 105
+//   38912 x 3072 x 768       7.13    124 / 141 / 100       116 / 138 / 96.5
+//   38912 x 3072 x 1536      7.13    204 / 214 / 178       186 / 201 / 167
+//   16384 x 4096 x 4096      4.00    272 / 263 / 245       231 / 232 / 213
+// and to 8 bits with GELU, three sets of operands in turn:
+//   12928 x 1024 x 1024      0.80    24.4                  22.7
+//   9728 x 3072 x 768        1.78    40.4                  37.1
+//   25856 x 1024 x 1024      1.58    45.1                  41.9
+//   51712 x 1024 x 512       3.16    55.9                  57.4
+//   103424 x 1024 x 1024     6.31    158                   145
+//   38912 x 3072 x 384       7.13    99.4                  99.3
+//   38912 x 3072 x 768       7.13    135-148               134-143
+//   38912 x 3072 x 1536      7.13    216                   209
 template <Out OUT, bool SF>
 void launch_best(const GemmArgs& a, hipStream_t stream) {
   const int m = a.m, n = a.n, k = a.k;
@@ -1044,11 +1061,10 @@ void launch_best(const GemmArgs& a, hipStream_t stream) {
   if (tiles(128, 64) <= kUnits) return launch_tiles<1, 4, 1, 2, OUT, SF>(a, stream);
   if (tiles(128, 64) <= 2 * kUnits) return launch_tiles<1, 4, 1, 1, OUT, SF>(a, stream);
   if constexpr (!kExact<OUT, SF>) {
-    // 256 x 256 where workgroups come out about even, but not for GELU to 8 bits of a
-    // short shared axis: nothing runs beside its results' work
+    // 256 x 256 where workgroups come out about even
     const long wide = tiles(256, 256), rounds = (wide + kUnits - 1) / kUnits;
     if (k % kBlock == 0 && k >= 2 * kBlock && n % kBlock == 0 && n >= 256 && m >= 256 &&
-        4 * wide >= 3 * rounds * kUnits && !(OUT == kFp8 && a.gelu && k < 2048))
+        4 * wide >= 3 * rounds * kUnits)
       return launch_wide<OUT, SF>(a, stream);
     // 256 x 128 goes round twice a unit at a time: the last round has to be worth it
     const long large = tiles(256, 128), round = 2 * kUnits;
