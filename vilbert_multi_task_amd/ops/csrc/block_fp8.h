@@ -65,13 +65,15 @@ DEV unsigned int pack2_bf16(float a, float b) {
 }
 
 // the scale of a block, as it is held in f32 or in bf16, from its largest value
-DEV float block_scale(float amax, bool f32) {
+template <bool F32>
+DEV float block_scale(float amax) {
   const float s = fmaxf(amax / 448.0f, 0x1p-100f);
-  return f32 ? s : us2f((unsigned short)pack2_bf16(s, s));
+  return F32 ? s : us2f((unsigned short)pack2_bf16(s, s));
 }
 // number i of `scales`, of block_scale: nothing to round
-DEV void store_scale(void* scales, long i, float scale, bool f32) {
-  if (f32)
+template <bool F32>
+DEV void store_scale(void* scales, long i, float scale) {
+  if (F32)
     ((float*)scales)[i] = scale;
   else
     ((unsigned short*)scales)[i] = (unsigned short)(__float_as_uint(scale) >> 16);

@@ -34,12 +34,11 @@ struct NormArgs {
   const T *x, *res, *w, *b;
   T *y, *sum;
   unsigned char* y8;
-  void* scales;  // bf16, or f32 where scales_f32
+  void* scales;  // f32 by the kernels that are SF, else bf16
   float* rstd;
   long rows;
   int dim;
   float eps;
-  bool scales_f32;
 };
 
 // us for 103424 rows of 1024 in bf16 (TB/s of what has to be moved): rms with the
@@ -49,7 +48,10 @@ struct NormArgs {
 // t = x + res; rms: y = t / sqrt(mean t^2 + eps) * w with t as the type holds
 // it (it is the stream that goes on), layer: y = (t - mean) / sqrt(var + eps)
 // * w + b with t in 32 bits.
-template <typename T, Form FORM, bool RES, int L, int R>
+//
+// The type of the scales is the kernel's (SF): asked for at run time it takes six
+// registers, and the layer norm of 1024 one wave less a SIMD (111 us became 113).
+template <typename T, Form FORM, bool RES, bool SF, int L, int R>
 __global__ __launch_bounds__(threads_of(L)) void block_norm_kernel(
     NormArgs<T> a) {
   constexpr int kRowsPerBlock = threads_of(L) / L;
@@ -120,12 +122,12 @@ __global__ __launch_bounds__(threads_of(L)) void block_norm_kernel(
       }
       if (FORM != kRms8) store8_row(a.y + row * dim, j, dim, y);
       if (FORM != kRms) {
-        const float scale = block_scale(group16_max(absmax<8>(y)), a.scales_f32);
+        const float scale = block_scale<SF>(group16_max(absmax<8>(y)));
         if (j < dim) {
           *reinterpret_cast<uint2*>(a.y8 + row * pitch + j) =
               pack8_block(y, 1.0f / scale);
           if ((t & 15) == 0)
-            store_scale(a.scales, row * groups + j / kBlock, scale, a.scales_f32);
+            store_scale<SF>(a.scales, row * groups + j / kBlock, scale);
         }
       }
     }
@@ -134,10 +136,10 @@ __global__ __launch_bounds__(threads_of(L)) void block_norm_kernel(
 
 // rows in blocks of 128: 16 lanes a block, no block needs another (103424 rows of
 // 1024 in bf16: 59 us, 5.4 TB/s)
-template <typename T>
+template <typename T, bool SF>
 __global__ __launch_bounds__(256) void quantize_block_kernel(
     const T* __restrict__ x, unsigned char* __restrict__ y8,
-    void* __restrict__ scales, bool scales_f32, long rows, int dim) {
+    void* __restrict__ scales, long rows, int dim) {
   const int groups = ceil_div(dim, kBlock);
   const long pitch = fp8_pitch(dim);
   const long n = rows * groups;
@@ -147,19 +149,19 @@ __global__ __launch_bounds__(256) void quantize_block_kernel(
     const int j = (int)(g - row * groups) * kBlock + (threadIdx.x & 15) * 8;
     float v[8];
     load8_row(x + row * dim, j, dim, v);
-    const float scale = block_scale(group16_max(absmax<8>(v)), scales_f32);
+    const float scale = block_scale<SF>(group16_max(absmax<8>(v)));
     if (j < dim)
       *reinterpret_cast<uint2*>(y8 + row * pitch + j) = pack8_block(v, 1.0f / scale);
-    if ((threadIdx.x & 15) == 0) store_scale(scales, g, scale, scales_f32);
+    if ((threadIdx.x & 15) == 0) store_scale<SF>(scales, g, scale);
   }
 }
 
 // a weight in blocks of 128 x 128: a workgroup a block, 8 rows of 16 values a
 // thread's share, held in registers between the two passes
-template <typename T>
+template <typename T, bool SF>
 __global__ __launch_bounds__(256) void quantize_block_weight_kernel(
     const T* __restrict__ w, unsigned char* __restrict__ w8,
-    void* __restrict__ scales, bool scales_f32, int n, int k) {
+    void* __restrict__ scales, int n, int k) {
   __shared__ float lds[4];
   const long pitch = fp8_pitch(k);
   const int j = blockIdx.x * kBlock + (threadIdx.x & 15) * 8;
@@ -178,7 +180,7 @@ __global__ __launch_bounds__(256) void quantize_block_weight_kernel(
   if (lane_id() == 0) lds[wave_id()] = a;
   __syncthreads();
   const float scale =
-      block_scale(fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3])), scales_f32);
+      block_scale<SF>(fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3])));
   const float inv = 1.0f / scale;
 #pragma unroll
   for (int r = 0; r < 8; ++r) {
@@ -187,7 +189,7 @@ __global__ __launch_bounds__(256) void quantize_block_weight_kernel(
       *reinterpret_cast<uint2*>(w8 + row * pitch + j) = pack8_block(v[r], inv);
   }
   if (threadIdx.x == 0)
-    store_scale(scales, (long)blockIdx.y * gridDim.x + blockIdx.x, scale, scales_f32);
+    store_scale<SF>(scales, (long)blockIdx.y * gridDim.x + blockIdx.x, scale);
 }
 
 // Backward of y = n * w, n = t * rstd:  h = gy * w,  c = mean(h * n),
@@ -299,13 +301,13 @@ int rows_at_once(int dim) {
   return dim <= 128 ? 16 : dim <= 256 ? 8 : dim <= 2048 ? 4 : 1;
 }
 
-template <typename T, Form FORM, bool RES, int L, int R>
+template <typename T, Form FORM, bool RES, bool SF, int L, int R>
 void norm_launch(const NormArgs<T>& a, hipStream_t stream) {
   constexpr int rows = threads_of(L) / L;
   const long blocks = (a.rows + rows - 1) / rows;
   // a launch has fewer than 2^32 threads
   const int grid = (int)(blocks < (1 << 21) ? blocks : (1 << 21));
-  hipLaunchKernelGGL((block_norm_kernel<T, FORM, RES, L, R>), dim3(grid),
+  hipLaunchKernelGGL((block_norm_kernel<T, FORM, RES, SF, L, R>), dim3(grid),
                      dim3(threads_of(L)), 0, stream, a);
 }
 
@@ -325,11 +327,21 @@ void norm_launch(const NormArgs<T>& a, hipStream_t stream) {
     else LAUNCH(1024, 8);                   \
   } while (0)
 
-template <typename T, Form FORM, bool RES>
+template <typename T, Form FORM, bool RES, bool SF>
 void norm_by_width(const NormArgs<T>& a, hipStream_t stream) {
-#define LAUNCH(L, R) norm_launch<T, FORM, RES, L, R>(a, stream)
+#define LAUNCH(L, R) norm_launch<T, FORM, RES, SF, L, R>(a, stream)
   BY_WIDTH(a.dim, LAUNCH);
 #undef LAUNCH
+}
+template <typename T, Form FORM>
+void norm_by_kind(const NormArgs<T>& a, bool scales_f32, hipStream_t stream) {
+  if constexpr (FORM != kRms) {
+    if (scales_f32)
+      return a.res ? norm_by_width<T, FORM, true, true>(a, stream)
+                   : norm_by_width<T, FORM, false, true>(a, stream);
+  }
+  a.res ? norm_by_width<T, FORM, true, false>(a, stream)
+        : norm_by_width<T, FORM, false, false>(a, stream);
 }
 
 }  // namespace
@@ -341,17 +353,13 @@ void launch_block_norm(int form, const T* x, const T* res, const T* w,
                        const T* b, T* y, T* sum, unsigned char* y8,
                        void* scales, bool scales_f32, float* rstd, long rows,
                        int dim, float eps, hipStream_t stream) {
-  const NormArgs<T> a{x,    res,  w,   b,   y,  sum,
-                      y8, scales, rstd, rows, dim, eps, scales_f32};
+  const NormArgs<T> a{x, res, w, b, y, sum, y8, scales, rstd, rows, dim, eps};
   if (form == 0)
-    res ? norm_by_width<T, kRms, true>(a, stream)
-        : norm_by_width<T, kRms, false>(a, stream);
+    norm_by_kind<T, kRms>(a, scales_f32, stream);
   else if (form == 1)
-    res ? norm_by_width<T, kRms8, true>(a, stream)
-        : norm_by_width<T, kRms8, false>(a, stream);
+    norm_by_kind<T, kRms8>(a, scales_f32, stream);
   else
-    res ? norm_by_width<T, kLayer8, true>(a, stream)
-        : norm_by_width<T, kLayer8, false>(a, stream);
+    norm_by_kind<T, kLayer8>(a, scales_f32, stream);
 }
 
 // How many rows of partial sums launch_rms_bwd writes: four workgroups a compute
@@ -391,18 +399,26 @@ void launch_quantize_block(const T* x, unsigned char* y8, void* scales,
                            bool scales_f32, long rows, int dim,
                            hipStream_t stream) {
   const long blocks = (rows * ceil_div(dim, kBlock) + 15) / 16;
-  hipLaunchKernelGGL((quantize_block_kernel<T>),
-                     dim3((int)(blocks < 8192 ? blocks : 8192)), dim3(256), 0,
-                     stream, x, y8, scales, scales_f32, rows, dim);
+  const dim3 grid((int)(blocks < 8192 ? blocks : 8192));
+  if (scales_f32)
+    hipLaunchKernelGGL((quantize_block_kernel<T, true>), grid, dim3(256), 0, stream, x,
+                       y8, scales, rows, dim);
+  else
+    hipLaunchKernelGGL((quantize_block_kernel<T, false>), grid, dim3(256), 0, stream, x,
+                       y8, scales, rows, dim);
 }
 
 template <typename T>
 void launch_quantize_block_weight(const T* w, unsigned char* w8, void* scales,
                                   bool scales_f32, int n, int k,
                                   hipStream_t stream) {
-  hipLaunchKernelGGL((quantize_block_weight_kernel<T>),
-                     dim3(ceil_div(k, kBlock), ceil_div(n, kBlock)), dim3(256),
-                     0, stream, w, w8, scales, scales_f32, n, k);
+  const dim3 grid(ceil_div(k, kBlock), ceil_div(n, kBlock));
+  if (scales_f32)
+    hipLaunchKernelGGL((quantize_block_weight_kernel<T, true>), grid, dim3(256), 0,
+                       stream, w, w8, scales, n, k);
+  else
+    hipLaunchKernelGGL((quantize_block_weight_kernel<T, false>), grid, dim3(256), 0,
+                       stream, w, w8, scales, n, k);
 }
 
 #define INSTANTIATE(T)                                                        \

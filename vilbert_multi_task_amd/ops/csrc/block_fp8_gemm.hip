@@ -637,7 +637,7 @@ block_gemm_tile_kernel(GemmArgs a, int mtiles, int ntiles) {
       float most = absmax<32>(v);
       most = fmaxf(most, __shfl_xor(most, 16));
       most = fmaxf(most, __shfl_xor(most, 32));
-      const float scale = block_scale(most, SF), inv = 1.0f / scale;
+      const float scale = block_scale<SF>(most), inv = 1.0f / scale;
 #pragma unroll
       for (int g = 0; g < 4; ++g)
         *reinterpret_cast<uint2*>(out + row * 128 +
@@ -645,7 +645,7 @@ block_gemm_tile_kernel(GemmArgs a, int mtiles, int ntiles) {
             pack8_block(v + 8 * g, inv);
       const int m = m0 + wm * MT * 16 + row;
       if (q == 0 && m < a.m)
-        store_scale(a.ys, (long)m * groups + nw / kBlock, scale, SF);
+        store_scale<SF>(a.ys, (long)m * groups + nw / kBlock, scale);
     }
   }
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -970,13 +970,13 @@ __global__ __launch_bounds__(512, 2) void block_gemm_wide_kernel(GemmArgs a, int
           float most = absmax<32>(v);
           most = fmaxf(most, __shfl_xor(most, 16));
           most = fmaxf(most, __shfl_xor(most, 32));
-          const float scale = block_scale(most, false), inv = 1.0f / scale;
+          const float scale = block_scale<SF>(most), inv = 1.0f / scale;
 #pragma unroll
           for (int g = 0; g < 4; ++g)
             *reinterpret_cast<uint2*>(out + re * 128 + (((g * 2 + qe / 2) ^ (re & 7)) << 4) +
                                       (qe & 1) * 8) = pack8_block(v + 8 * g, inv);
           if (qe == 0 && m + re >= own_m)
-            store_scale(a.ys, (long)(m + re) * groups + nw / kBlock, scale, false);
+            store_scale<SF>(a.ys, (long)(m + re) * groups + nw / kBlock, scale);
           leave((unsigned char*)a.y + nw, a.n);
         }
         __builtin_amdgcn_sched_barrier(0);
