@@ -294,3 +294,20 @@ def test_switches_are_read_as_they_are_at_the_call(monkeypatch):
                 call()
                 assert ("vilbert_amd::" + op in seen.names) == own, (name, value, op)
             env.pop(name)
+
+
+@gpu
+def test_compiled_whole():
+    """Nothing in the entry points breaks a compiled graph."""
+    x, w, _, _, p = _args("cuda")
+
+    def step(x, w, *p):
+        q, s = F_ops.rms_norm_fp8_block(x, w, EPS)
+        y = F_ops.rms_norm(x, w, EPS)
+        return q.float(), s, y, F_ops.fp8_block_linear(q, s, p[2], p[3], gelu=True), *F_ops.quantize_fp8_block(y)
+
+    with torch.no_grad():
+        want = step(x, w, *p)
+        got = torch.compile(step, backend="aot_eager", fullgraph=True)(x, w, *p)
+    for g, t in zip(got, want):
+        assert g.dtype == t.dtype and torch.equal(g.float(), t.float())

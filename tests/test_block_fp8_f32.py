@@ -385,3 +385,20 @@ def test_scales_whose_product_passes_the_range(m, n, k, device):
     xs[3, 0] = math.nan  # a scale that is none is not hidden
     assert torch.isnan(F_ops.fp8_block_linear(x8, xs, w8, ws, b)[3]).all()
     assert torch.isnan(F_ops.fp8_block_linear(x8, xs, w8, ws, b, out_dtype=F32)[3]).all()
+
+
+@gpu
+@pytest.mark.parametrize("m", [1, 40, 300, 2000, 8192])  # kernels of few, some, many and very many rows
+def test_gelu_to_bf16(m):
+    """Of a bias alone: 2^-17 of its value down to -4, 2^-14 down to -6, 2^-10 down to -8,
+    and an absolute error of 1e-14 below, each before bf16's half step."""
+    n = 8192
+    b = torch.linspace(-15, 15, n)
+    x8, w8 = torch.zeros(m, 256, device="cuda").to(E4), torch.zeros(n, 256, device="cuda").to(E4)
+    xs, ws = torch.ones(m, 2, device="cuda", dtype=BF), torch.ones(n // 128, 2, device="cuda", dtype=BF)
+    y = F_ops.fp8_block_linear(x8, xs, w8, ws, b.cuda(), gelu=True)[-1].cpu().to(F64)
+    v = b.to(F64)
+    y64 = v * 0.5 * torch.erfc(-v / math.sqrt(2))
+    tol = torch.where(v >= -4, 2.0 ** -17, torch.where(v >= -6, 2.0 ** -14, 2.0 ** -10)) * y64.abs()
+    tol = torch.where(v >= -8, tol, 1e-14)
+    assert ((y - y64).abs() <= tol + 2.0 ** -8 * (y64.abs() + tol)).all()

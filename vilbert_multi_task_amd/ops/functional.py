@@ -676,13 +676,16 @@ def fp8_block_linear(
     gelu: bool = False,
     out_dtype: torch.dtype = torch.bfloat16,
 ) -> torch.Tensor:
-    """y [..., N] (bf16/f32) = x @ w.T (+ bias), then exact (erf) GELU if `gelu`, of
+    """y [..., N] (bf16/f32) = x @ w.T (+ bias), then GELU (of erf) if `gelu`, of
     x8 [..., K] with scales [..., ceil(K/128)] and w8 [N, K] with scales
     [ceil(N/128), ceil(K/128)], both bf16 or both f32. Accumulated in f32 block by
     block, rounded once; bias is bf16/f32. To bf16 the products within a block are
     good to some 3e-5 of y (its 2-norm), to f32 they are exact and take twice as long.
     The product of two scales is one of f32's normal numbers: on the GPU a larger one is
     taken as the largest of them, a smaller one may be taken as 0.
+    GELU's own value is good to 2^-17 of itself down to -4 and to 2^-14 down to -6; below
+    -8, where it is less than 1e-14, only the absolute error is small. To f32 it is good
+    to 2^-18 down to -4, 2^-15 down to -8 and 2^-9 down to -12.9.
     Rows at a common distance that is a multiple of 16 bytes are read where they lie,
     others are copied."""
     f32 = _is_f32("fp8_block_linear", "out_dtype", out_dtype)
@@ -702,7 +705,7 @@ def fp8_block_linear_fp8(
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """fp8_block_linear whose y leaves in 8 bits, quantised from its f32
     values: (y8 [..., N], scales [..., ceil(N/128)] in the type of the others).
-    Where scales are f32 the products are exact, as for an f32 y."""
+    Where scales are f32 the products are exact, and GELU is, as for an f32 y."""
     if _serve_hip("fp8_block_linear_fp8", x8, x_scales, w8, w_scales, bias):
         return _EXT.fp8_block_linear_fp8(x8, x_scales, w8, w_scales, bias, gelu)
     return _quantize_block_ref(_block_linear_ref(
