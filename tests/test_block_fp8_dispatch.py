@@ -132,8 +132,12 @@ def test_refusals_of_fake_tensors():
         x, w, b, wide, p = _args("cuda")
         with pytest.raises(RuntimeError, match="rms_norm"):
             F_ops.rms_norm(x, w[:7], EPS)
-        with pytest.raises(RuntimeError, match="quantize_fp8_block"):
-            F_ops.quantize_fp8_block(x.half())
+        for t in (x.half(), x.double()):  # 64 bits: the plain form alone
+            with pytest.raises(RuntimeError, match="quantize_fp8_block"):
+                F_ops.quantize_fp8_block(t)
+            for res in (None, t):
+                with pytest.raises(RuntimeError, match="rms_norm"):
+                    F_ops.rms_norm(t, w.to(t.dtype), EPS, residual=res)
         with pytest.raises(RuntimeError, match="fp8_block_linear"):
             F_ops.fp8_block_linear(*p[:3], p[3][:1])
         with pytest.raises(RuntimeError, match="no gradient"):

@@ -28,18 +28,23 @@ def _like(x):
     return x.new_empty(x.shape)
 
 
+def _check_rms(x, w, res):
+    F_ops._check_rows("rms_norm", x)  # its plain form takes 64 bits too
+    F_ops._check_norm("rms_norm", x, w, res)
+
+
 def _rms_norm(x, w, eps):
-    F_ops._check_norm("rms_norm", x, w, None)
+    _check_rms(x, w, None)
     return _like(x)
 
 
 def _rms_norm_residual(x, res, w, eps):
-    F_ops._check_norm("rms_norm", x, w, res)
+    _check_rms(x, w, res)
     return _like(x), _like(x)
 
 
 def _rms_fwd_train(x, res, w, eps):
-    F_ops._check_norm("rms_norm", x, w, res)
+    _check_rms(x, w, res)
     total = x.new_empty((0,)) if res is None else _like(x)
     return _like(x), total, x.new_empty((x.numel() // x.shape[-1],), dtype=torch.float32)
 

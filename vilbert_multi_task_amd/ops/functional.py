@@ -533,7 +533,9 @@ def rms_norm(
     (y, t) is returned. bf16/f32, rows of up to 65536 values; statistics are
     f32 and y is rounded once. Gradients reach x, weight and residual, once;
     the weight's is added up in a fixed order, so the same inputs give the same
-    bits. Tensors with a forward-mode tangent are refused on the GPU."""
+    bits. Tensors with a forward-mode tangent are refused on the GPU. A backward pass
+    that is captured into a graph must not share leaves with an eager graph that is still
+    alive: torch would wait for the eager stream inside the capture."""
     if x.is_cuda and os.environ.get("VILBERT_AMD_FORCE_EAGER") != "1" and not (
         torch.is_grad_enabled() and os.environ.get("VILBERT_AMD_EAGER_BWD") == "1"
     ):
