@@ -25,10 +25,14 @@ benchmark keeps the reference-grade bf16 path.
 A second mode, ``convert_encoder_to_fp8_block`` (GraphRunner(fp8="block") /
 bench.py --fp8-block), has one scale per 128 values, taken from the values
 themselves (ops.functional's ``*_fp8_block``): no state between calls, no
-warm-up steps, an outlier costs only its own block, and the same request gives
-the same bits whenever it is repeated. LayerNorm emits its 8-bit form beside
-the bf16 one (``_fp8b`` on the result), and a feed-forward's intermediate
-leaves the first product in 8 bits, GELU applied, and never exists otherwise.
+warm-up steps, an outlier costs only its own block, and the same batch gives
+the same bits whenever it is repeated. (A request in a batch of another size may
+meet another kernel, which adds in another order; the last bit of a sum can move
+an 8-bit value by a step.) LayerNorm emits its 8-bit form beside the bf16 one
+(``_fp8b`` on the result), and a feed-forward's intermediate leaves the first
+product in 8 bits, GELU applied, and never exists otherwise. Convert where the
+model is served: the fused projections' weights stay on the device that they
+were made on.
 """
 
 from __future__ import annotations

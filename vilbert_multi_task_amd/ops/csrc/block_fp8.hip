@@ -42,7 +42,7 @@ struct NormArgs {
 };
 
 // us for 103424 rows of 1024 in bf16 (TB/s of what has to be moved): rms with the
-// residual to 8 bits 138 (5.3), layer to both 111 (4.8), rms 78 (5.4); a copy of
+// residual to 8 bits 135 (5.5), layer to both 111 (4.8), rms 78 (5.4); a copy of
 // 2 GiB runs at 4.8.
 //
 // t = x + res; rms: y = t / sqrt(mean t^2 + eps) * w with t as the type holds

@@ -170,8 +170,8 @@ DEV void store4(bf16* p, const float* v) {
   *reinterpret_cast<B16x4*>(p) = {{pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3])}};
 }
 // Results go past the caches: kept there, a round of tiles' results would fill an
-// XCD's whole cache and push out the W that the next round reads (103424x1024x1024:
-// 169 us with plain stores, 134 with these).
+// XCD's whole cache and push out the W that the next round reads (103424x1024x1024
+// by 256 x 128: 169 us with plain stores, 134 with these).
 DEV void store16_past(void* p, uint4 v) {  // at any multiple of 2 bytes
   typedef unsigned int u32x4 __attribute__((ext_vector_type(4), aligned(2)));
   __builtin_nontemporal_store(u32x4{v.x, v.y, v.z, v.w}, (u32x4*)p);
@@ -698,7 +698,7 @@ void launch_tiles(const GemmArgs& a, hipStream_t stream) {
 // Nothing that the compiler would wait for itself is loaded from memory on the way:
 // the scales and the bias come through shared memory as well. What bounds it then is
 // power: at 70% of the matrix unit's time the clock is down to 1.6 GHz of 2.4.
-// 8192x8192x8192 428 us (2570 TFLOP/s; 256 x 128 500), 103424x1024x1024 119 (1820).
+// 8192x8192x8192 447 us (2460 TFLOP/s; 256 x 128 515), 103424x1024x1024 126 (1720).
 //
 // Shared memory: two buffers of W and of X, two each of the rows' and W's scales
 // and of the bias, and room for results on their way out.
@@ -1006,18 +1006,19 @@ void launch_direct(const GemmArgs& a, hipStream_t stream) {
 }
 
 // The larger the tile the less is read for each result, as long as every compute
-// unit has a workgroup or two. us with bias to bf16 ("x2": two teams):
+// unit has a workgroup or two. us a call with bias to bf16, one call over and over in a
+// graph ("x2": two teams):
 //   rows x width x shared  direct 16x32  32x64  tiles 128x64 x2  128x64  128x128  256x128
-//   38 x 768 x 768                  3.7    4.9              6.0     5.9      7.8     10.6
-//   38 x 8192 x 4096               26     16               20      26       31       40
-//   256 x 1601 x 1024              10      7.0              7.6     8.0     10.6     14.9
-//   608 x 768 x 3072               23     14               12      15       21       29
-//   1616 x 1601 x 1024             45     33               11      10       11       16
-//   6464 x 3072 x 768                                      36      28       24       26
-//   16384 x 1024 x 1024                                            27       30       23
-//   103424 x 1024 x 1024                                          157      139      128
-// That is one call over and over, its operands in the caches. Of few rows what counts
-// is where W comes from; with other weights each call (60 MB of them), as in a model:
+//   38 x 768 x 768                  3.8    5.1              6.0     6.1      7.7     10.3
+//   38 x 8192 x 4096               28     17               21      28       33       40
+//   256 x 1601 x 1024              11      7.5              8.2     8.6     10.9     14.8
+//   608 x 768 x 3072               25     16               14      17       22       29
+//   1616 x 1601 x 1024             50     37               15      14       15       19
+//   6464 x 3072 x 768                                      40      32       27       30
+//   16384 x 1024 x 1024                                            32       29       26
+//   103424 x 1024 x 1024                                          176      140      126
+// Of few rows what counts is where W comes from. With other weights each call (60 MB of
+// them), as in a model, instead of the caches:
 //   38 x 8192 x 4096               29     18               21      28
 //   256 x 1601 x 1024              11      7.7              9.1    10.3
 //   608 x 768 x 1024               10      6.7              8.4     9.4
@@ -1025,27 +1026,21 @@ void launch_direct(const GemmArgs& a, hipStream_t stream) {
 //   1024 x 512 x 4096              32     18.6             20.1    25.8
 // so that the direct kernel has them, also where two teams are faster in a loop.
 //
-// Tiles of 256 x 256 in turn with the best of the others; rounds of 256 tiles, to
-// bf16 / to bf16 with GELU / to 8 bits, one call over and over:
-//   rows x width x shared   rounds  others                256 x 256
-//   9728 x 768 x 3072        0.45    34.0 / 35.6 / 32.5    39.9 / 43.4 / 38.0
-//   12928 x 1024 x 1024      0.80    24.7 / 28.6 / 24.2    20.7 / 24.6 / 19.1
-//   6464 x 3072 x 768        1.22    25.3 / 29.9 / 23.4    29.6 / 37.2 / 27.5
-//   9728 x 3072 x 768        1.78    35.3 / 43.2 / 32.1    33.8 / 39.9 / 29.0
-//   38912 x 768 x 3072       1.78    106 / 102 / 88.0      95.1 / 89.9 / 77.8
-//   103424 x 1024 x 1024     6.31    136 / 146 / 110       128 / 140 / 105
-//   38912 x 3072 x 768       7.13    124 / 141 / 100       116 / 138 / 96.5
-//   38912 x 3072 x 1536      7.13    204 / 214 / 178       186 / 201 / 167
-//   16384 x 4096 x 4096      4.00    272 / 263 / 245       231 / 232 / 213
-// and to 8 bits with GELU, three sets of operands in turn:
-//   12928 x 1024 x 1024      0.80    24.4                  22.7
-//   9728 x 3072 x 768        1.78    40.4                  37.1
-//   25856 x 1024 x 1024      1.58    45.1                  41.9
-//   51712 x 1024 x 512       3.16    55.9                  57.4
-//   103424 x 1024 x 1024     6.31    158                   145
-//   38912 x 3072 x 384       7.13    99.4                  99.3
-//   38912 x 3072 x 768       7.13    135-148               134-143
-//   38912 x 3072 x 1536      7.13    216                   209
+// Tiles of 256 x 256 and the best of the others, by rounds of 256 tiles; one call over
+// and over in a graph, to bf16 / to bf16 with GELU / to 8 bits / to 8 bits with GELU:
+//   rows x width x shared   rounds  others                       256 x 256
+//   9728 x 768 x 3072        0.45    36.3 / 37.4 / 35.1 / 37.6   40.8 / 43.6 / 40.0 / 44.0
+//   12928 x 1024 x 1024      0.80    22.9 / 27.9 / 23.2 / 27.7   23.2 / 26.5 / 21.9 / 26.5
+//   6464 x 3072 x 768        1.22    27.8 / 32.2 / 27.3 / 33.6   32.4 / 38.9 / 31.4 / 39.8
+//   9728 x 3072 x 768        1.78    37.0 / 45.3 / 35.6 / 43.7   35.0 / 41.7 / 32.5 / 41.3
+//   38912 x 768 x 3072       1.78    95.8 / 106 / 96.4 / 102     87.9 / 96.3 / 86.6 / 95.3
+//   16384 x 4096 x 4096      4.00    269 / 292 / 276 / 284       237 / 249 / 238 / 257
+//   103424 x 1024 x 1024     6.31    132 / 160 / 126 / 149       126 / 148 / 116 / 148
+//   38912 x 3072 x 768       7.13    117 / 153 / 116 / 139       111 / 139 / 109 / 140
+//   38912 x 3072 x 1536      7.13    208 / 234 / 202 / 227       195 / 219 / 186 / 220
+// and to 8 bits with GELU, three sets of operands in turn, 103424 x 1024 x 1024 158 and
+// 145, 25856 x 1024 x 1024 45 and 42, 51712 x 1024 x 512 56 and 57, 38912 x 3072 x 384
+// 99 and 99; in the served encoder 162 and 149.
 template <Out OUT, bool SF>
 void launch_best(const GemmArgs& a, hipStream_t stream) {
   const int m = a.m, n = a.n, k = a.k;
