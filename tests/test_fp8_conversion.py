@@ -50,7 +50,8 @@ def _linears(model):
 
 @pytest.mark.parametrize("cast", [
     lambda m: m.to(torch.bfloat16), lambda m: m.bfloat16(), lambda m: m.half(), lambda m: m.double(),
-    lambda m: m.to("cpu"), lambda m: m.to(torch.bfloat16).float()])
+    lambda m: m.to("cpu"), lambda m: m.to(torch.bfloat16).float(), lambda m: m.type(torch.bfloat16),
+    lambda m: m.share_memory()])
 def test_casts_leave_8_bit_weights_and_their_scales(cast):
     model = _model()
     convert_encoder_to_fp8_block(model)

@@ -300,7 +300,10 @@ class BlockFp8Linear(nn.Module):
         held = {}
         for name, as_int in (("w8", torch.uint8), ("w_scales", torch.int16)):
             t = self._buffers[name]
-            held[name] = fn(t.view(as_int)).view(t.dtype)
+            moved = fn(t.view(as_int))
+            if moved.dtype != as_int:  # Module.type() casts whatever there is
+                moved = t.view(as_int).to(moved.device)
+            held[name] = moved.view(t.dtype)
         for name in held:
             del self._buffers[name]
         try:
